@@ -83,6 +83,7 @@ def lib() -> ctypes.CDLL:
             "fkc_kernel_find": (i32, [ctypes.c_char_p, u64, ctypes.POINTER(i32)]),
             "fkc_fnv1a64": (u64, [vp, sz]),
             "fkc_launch": (i32, [vp, i32, vp, sz, pvp, i32]),
+            "fkc_linear_mxfp4_work": (i32, [u32, u32, u32, u32, u32, ctypes.POINTER(sz)]),
             "fkc_capture_begin": (i32, [vp]),
             "fkc_capture_end": (i32, [vp, pvp]),
             "fkc_graph_launch": (i32, [vp, vp]),
@@ -147,8 +148,18 @@ class TableEntry:
     buffers: list = field(default_factory=list)
     params: list = field(default_factory=list)
 
+    def __post_init__(self):
+        # Every parameter is 4 bytes, so the struct has no gaps.
+        self._names = tuple(p.name for p in self.params)
+        self._struct = struct.Struct("<" + "".join({"u32": "I", "f32": "f", "i32": "i"}[p.type] for p in self.params))
+
     def pack(self, values: dict) -> bytes:
         """The parameter struct's bytes in C layout (Abi.hs:113-133)."""
+        if len(values) == len(self._names) and self._struct.size == self.params_size:
+            try:  # the usual call; a wrong name is worded below
+                return self._struct.pack(*[values[n] for n in self._names])
+            except KeyError:
+                pass
         buf = bytearray(self.params_size)
         names = {p.name for p in self.params}
         extra = set(values) - names
@@ -373,8 +384,7 @@ class Context:
             raise Refused(FKC_ERR_ARGUMENT, f"The target has no kernel {kernel}.")
         raw = e.pack(params)
         ptrs = (ctypes.c_void_p * len(bufs))(*[b.ptr if isinstance(b, DeviceBuffer) else int(b) for b in bufs])
-        pbuf = ctypes.create_string_buffer(raw, len(raw)) if raw else None
-        check(lib().fkc_launch(self.handle, e.id, pbuf, len(raw), ptrs, len(bufs)))
+        check(lib().fkc_launch(self.handle, e.id, raw or None, len(raw), ptrs, len(bufs)))
 
     def capture_begin(self) -> None:
         check(lib().fkc_capture_begin(self.handle))
@@ -405,6 +415,14 @@ class Context:
 
     def comm_destroy(self) -> None:
         check(lib().fkc_comm_destroy(self.handle))
+
+
+def linear_mxfp4_work(n: int, kk: int, m: int, entries: int = 1, k: int = 1) -> int:
+    """The bytes of the `work` buffer of linear_mxfp4 (entries 1, k 1) and
+    linear_routed_mxfp4 for these sizes, whatever their type."""
+    b = ctypes.c_size_t()
+    check(lib().fkc_linear_mxfp4_work(entries, n, kk, m, k, ctypes.byref(b)))
+    return b.value
 
 
 def pinned(shape, dtype) -> np.ndarray:

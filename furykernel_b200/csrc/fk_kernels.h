@@ -220,6 +220,35 @@ cudaError_t fk_launch_gemv_routed(const void* table, FkElem e, uint32_t entries,
 cudaError_t fk_launch_gated_gelu(const float* x, uint64_t segments, uint32_t f, float* y, bool pdl, cudaStream_t s);
 cudaError_t fk_launch_combine_ranks_add(const float* r, const float* ws, const float* segs, uint32_t m, uint32_t k,
                                         uint32_t d, float* y, bool pdl, cudaStream_t s);
+// The grouped router (k_route_grouped.cu).
+struct FkRouteGrouped {
+  const void* x;      // [m, ldx] router logits
+  const float* bias;  // [n] added to the scores where experts are compared, or null
+  uint32_t* ids;      // [m, k]
+  float* ws;          // [m, k]
+  uint32_t m, n, k, groups, top_groups, group_by, ldx;
+  bool sigmoid, renorm;
+  float factor;
+};
+cudaError_t fk_launch_route_grouped(const FkRouteGrouped& a, FkElem e, bool pdl, cudaStream_t s);
+// MXFP4 (fk_mxfp4.cuh): rows to codes and scales and back (k_mxfp4.cu), and
+// the products with such weights (k_linear_mxfp4.cu).
+cudaError_t fk_launch_quant_mxfp4(const void* x, FkElem e, uint64_t rows, uint32_t k, uint32_t ldx, uint8_t* codes,
+                                  uint8_t* scales, bool pdl, cudaStream_t s);
+cudaError_t fk_launch_widen_mxfp4(const uint8_t* codes, const uint8_t* scales, uint64_t rows, uint32_t k,
+                                  uint32_t ldy, void* y, FkElem e, bool pdl, cudaStream_t s);
+struct FkLinearMx {
+  const uint8_t* w;       // codes [entries, n, kk / 2]
+  const uint8_t* scales;  // [entries, n, kk / 32]
+  const uint32_t* ids;    // [m, k], or null: every pair takes entry 0
+  const void* x;          // [m, ldx]: one segment of kk every rank takes, or k of them
+  void* y;                // [m, ldy]: a segment of n a rank
+  void* work;             // fk_linear_mxfp4_work bytes
+  uint32_t entries, n, kk, m, k, ldx, ldy;
+  bool per_rank;
+};
+size_t fk_linear_mxfp4_work(uint64_t entries, uint64_t n, uint64_t kk, uint64_t m, uint64_t k);
+cudaError_t fk_launch_linear_mxfp4(const FkLinearMx& a, FkElem e, bool pdl, cudaStream_t s);
 cudaError_t fk_launch_rope_tables(float* cos_t, float* sin_t, double theta, uint32_t d, uint32_t rotated,
                                   uint32_t positions, cudaStream_t s);
 

@@ -997,6 +997,82 @@ int l_combine_ranks_add(fkc_ctx* c, const Params& p, void* const* bufs) {
                   "combine_ranks_add");
 }
 
+// ---- the grouped router and MXFP4 weights --------------------------------
+#define XN(base) (EL == FK_F32 ? base : EL == FK_BF16 ? base "_xbf16" : base "_xf16")
+
+// route_grouped: x ids ws | m n k groups top_groups group_by sigmoid renorm ldx factor;
+// route_grouped_bias: x bias ids ws | the same.
+template <FkElem EL, bool BIAS>
+int l_route_grouped(fkc_ctx* c, const Params& p, void* const* bufs) {
+  const char* name = BIAS ? XN("route_grouped_bias") : XN("route_grouped");
+  FkRouteGrouped a = {};
+  a.x = bufs[0];
+  a.bias = BIAS ? CF(1) : nullptr;
+  a.ids = U(BIAS ? 2 : 1);
+  a.ws = F(BIAS ? 3 : 2);
+  a.m = p.u(0), a.n = p.u(1), a.k = p.u(2), a.groups = p.u(3), a.top_groups = p.u(4), a.group_by = p.u(5);
+  a.sigmoid = p.u(6) != 0, a.renorm = p.u(7) != 0;
+  a.ldx = p.u(8);
+  a.factor = p.f(9);
+  if (a.n % a.groups != 0)
+    return fail(FKC_ERR_ARGUMENT, "%s: %u experts do not form %u groups.", name, a.n, a.groups);
+  if (a.top_groups > a.groups)
+    return fail(FKC_ERR_ARGUMENT, "%s: top_groups %u is more than the %u groups.", name, a.top_groups, a.groups);
+  if (a.k > a.top_groups * (a.n / a.groups))
+    return fail(FKC_ERR_ARGUMENT, "%s: k %u is more than the %u experts of %u groups.", name, a.k,
+                a.top_groups * (a.n / a.groups), a.top_groups);
+  if (a.ldx < a.n) return fail(FKC_ERR_ARGUMENT, "%s: ldx %u is less than n %u.", name, a.ldx, a.n);
+  return launched(fk_launch_route_grouped(a, EL, c->pdl, c->stream), name);
+}
+
+// quant_mxfp4: x codes scales | rows k ldx
+template <FkElem EL>
+int l_quant_mxfp4(fkc_ctx* c, const Params& p, void* const* bufs) {
+  const char* name = XN("quant_mxfp4");
+  if (p.u(2) < p.u(1)) return fail(FKC_ERR_ARGUMENT, "%s: ldx %u is less than k %u.", name, p.u(2), p.u(1));
+  return launched(fk_launch_quant_mxfp4(bufs[0], EL, p.u(0), p.u(1), p.u(2), (uint8_t*)bufs[1], (uint8_t*)bufs[2],
+                                        c->pdl, c->stream),
+                  name);
+}
+// widen_mxfp4: codes scales y | rows k ldy
+template <FkElem EL>
+int l_widen_mxfp4(fkc_ctx* c, const Params& p, void* const* bufs) {
+  const char* name = EL == FK_F32 ? "widen_mxfp4" : EL == FK_BF16 ? "widen_mxfp4_ybf16" : "widen_mxfp4_yf16";
+  if (p.u(2) < p.u(1)) return fail(FKC_ERR_ARGUMENT, "%s: ldy %u is less than k %u.", name, p.u(2), p.u(1));
+  return launched(fk_launch_widen_mxfp4((const uint8_t*)bufs[0], (const uint8_t*)bufs[1], p.u(0), p.u(1), p.u(2),
+                                        bufs[2], EL, c->pdl, c->stream),
+                  name);
+}
+
+int linear_mxfp4(fkc_ctx* c, const FkLinearMx& a, FkElem el, const char* name) {
+  const uint64_t xw = (uint64_t)a.kk * (a.per_rank ? a.k : 1), yw = (uint64_t)a.n * a.k;
+  if (a.ldx < xw)
+    return fail(FKC_ERR_ARGUMENT, "%s: ldx %u is less than a row's %llu inputs.", name, a.ldx, (unsigned long long)xw);
+  if (a.ldy < yw)
+    return fail(FKC_ERR_ARGUMENT, "%s: ldy %u is less than a row's %llu outputs.", name, a.ldy,
+                (unsigned long long)yw);
+  return launched(fk_launch_linear_mxfp4(a, el, c->pdl, c->stream), name);
+}
+// linear_mxfp4: w w_scale x y work | n k m ldx ldy
+template <FkElem EL>
+int l_linear_mxfp4(fkc_ctx* c, const Params& p, void* const* bufs) {
+  FkLinearMx a = {};
+  a.w = (const uint8_t*)bufs[0], a.scales = (const uint8_t*)bufs[1], a.x = bufs[2], a.y = bufs[3], a.work = bufs[4];
+  a.entries = 1, a.n = p.u(0), a.kk = p.u(1), a.m = p.u(2), a.k = 1, a.ldx = p.u(3), a.ldy = p.u(4);
+  return linear_mxfp4(c, a, EL, XN("linear_mxfp4"));
+}
+// linear_routed_mxfp4: table t_scale ids x y work | entries n kk m k ldx ldy per_rank
+template <FkElem EL>
+int l_linear_routed_mxfp4(fkc_ctx* c, const Params& p, void* const* bufs) {
+  FkLinearMx a = {};
+  a.w = (const uint8_t*)bufs[0], a.scales = (const uint8_t*)bufs[1], a.ids = CU(2);
+  a.x = bufs[3], a.y = bufs[4], a.work = bufs[5];
+  a.entries = p.u(0), a.n = p.u(1), a.kk = p.u(2), a.m = p.u(3), a.k = p.u(4), a.ldx = p.u(5), a.ldy = p.u(6);
+  a.per_rank = p.u(7) != 0;
+  return linear_mxfp4(c, a, EL, XN("linear_routed_mxfp4"));
+}
+#undef XN
+
 // ---- paged KV caches: each row's block table (indices), the blocks reached
 // through the caches' tables of block addresses (bound after the buffers,
 // as the reference's ABI orders tables: Abi.hs:136-159) -------------------
@@ -1408,6 +1484,50 @@ std::vector<KernelSpec> make_table() {
                {{"r", "read", "f32"}, {"ws", "read", "f32"}, {"segs", "read", "f32"}, {"y", "write", "f32"}},
                {dim("m", 1, 65535), dim("k", 1, 8), dim("d", 1, kMax)},
                l_combine_ranks_add});
+  // The grouped router and MXFP4 weights.
+  for (bool bias : {false, true}) {
+    std::vector<BufSpec> bufs = {{"x", "read", "f32"}};
+    if (bias) bufs.push_back({"bias", "read", "f32"});
+    bufs.push_back({"ids", "write", "u32"});
+    bufs.push_back({"ws", "write", "f32"});
+    t.push_back({bias ? "route_grouped_bias" : "route_grouped",
+                 128,
+                 bufs,
+                 {dim("m", 1, 1048576), dim("n", 1, 1024), dim("k", 1, 8), dim("groups", 1, 32),
+                  dim("top_groups", 1, 32), dim("group_by", 1, 2), dim("sigmoid", 0, 1), dim("renorm", 0, 1),
+                  u32("ldx"), f32("factor")},
+                 bias ? l_route_grouped<FK_F32, true> : l_route_grouped<FK_F32, false>});
+  }
+  t.push_back({"quant_mxfp4",
+               256,
+               {{"x", "read", "f32"}, {"codes", "write", "u8"}, {"scales", "write", "u8"}},
+               {dim("rows", 1, 268435456), dim("k", 32, 1048576, 32), u32("ldx")},
+               l_quant_mxfp4<FK_F32>});
+  t.push_back({"widen_mxfp4",
+               256,
+               {{"codes", "read", "u8"}, {"scales", "read", "u8"}, {"y", "write", "f32"}},
+               {dim("rows", 1, 268435456), dim("k", 32, 1048576, 32), u32("ldy")},
+               l_widen_mxfp4<FK_F32>});
+  t.push_back({"linear_mxfp4",
+               256,
+               {{"w", "read", "u8"},
+                {"w_scale", "read", "u8"},
+                {"x", "read", "f32"},
+                {"y", "write", "f32"},
+                {"work", "read_write", "u8"}},
+               {dim("n", 1, 1048576), dim("k", 32, 65536, 32), dim("m", 1, 65535), u32("ldx"), u32("ldy")},
+               l_linear_mxfp4<FK_F32>});
+  t.push_back({"linear_routed_mxfp4",
+               256,
+               {{"table", "read", "u8"},
+                {"t_scale", "read", "u8"},
+                {"ids", "read", "u32"},
+                {"x", "read", "f32"},
+                {"y", "write", "f32"},
+                {"work", "read_write", "u8"}},
+               {dim("entries", 1, 4096), dim("n", 1, 1048576), dim("kk", 32, 65536, 32), dim("m", 1, 65535),
+                dim("k", 1, 8), u32("ldx"), u32("ldy"), dim("per_rank", 0, 1)},
+               l_linear_routed_mxfp4<FK_F32>});
   // The 16-bit forms: an f32 entry's parameters with some buffers bf16 or
   // f16 (the model's weights, or its KV caches) and their own launchers.
   struct Variant {
@@ -1425,6 +1545,11 @@ std::vector<KernelSpec> make_table() {
   {base, base "_kvbf16", {"k_cache", "v_cache"}, fn<FK_BF16>, "bf16"}, {          \
     base, base "_kvf16", {"k_cache", "v_cache"}, fn<FK_F16>, "f16"                \
   }
+#define X_FORMS(base, bf16, f16, ...)                        \
+  {base, base "_xbf16", {__VA_ARGS__}, bf16, "bf16"}, {      \
+    base, base "_xf16", {__VA_ARGS__}, f16, "f16"            \
+  }
+#define X_FORMS_OF(base, fn, ...) X_FORMS(base, fn<FK_BF16>, fn<FK_F16>, __VA_ARGS__)
   const std::vector<Variant> variants = {
       W_FORMS("gemv", l_gemv_w16, "w"),
       W_FORMS("gemv_add", l_gemv_add_w16, "w"),
@@ -1440,6 +1565,13 @@ std::vector<KernelSpec> make_table() {
       W_FORMS("split_tf32", l_split_tf32_w16, "x"),
       W_FORMS("gemv_routed", l_gemv_routed_w16, "table"),
       W_FORMS("route_topk_scaled", l_route_topk_scaled_w16, "scale"),
+      X_FORMS("route_grouped", (l_route_grouped<FK_BF16, false>), (l_route_grouped<FK_F16, false>), "x"),
+      X_FORMS("route_grouped_bias", (l_route_grouped<FK_BF16, true>), (l_route_grouped<FK_F16, true>), "x"),
+      X_FORMS_OF("quant_mxfp4", l_quant_mxfp4, "x"),
+      X_FORMS_OF("linear_mxfp4", l_linear_mxfp4, "x", "y"),
+      X_FORMS_OF("linear_routed_mxfp4", l_linear_routed_mxfp4, "x", "y"),
+      {"widen_mxfp4", "widen_mxfp4_ybf16", {"y"}, l_widen_mxfp4<FK_BF16>, "bf16"},
+      {"widen_mxfp4", "widen_mxfp4_yf16", {"y"}, l_widen_mxfp4<FK_F16>, "f16"},
       KV_FORMS("kv_store_ring", l_kv_store_kv16),
       KV_FORMS("attend_split", l_attend_kv16),
       KV_FORMS("attend_decode", l_attend_decode_kv16),
@@ -1451,6 +1583,8 @@ std::vector<KernelSpec> make_table() {
   };
 #undef W_FORMS
 #undef KV_FORMS
+#undef X_FORMS
+#undef X_FORMS_OF
   for (const Variant& v : variants) {
     KernelSpec k;
     bool found = false;
@@ -1576,6 +1710,13 @@ extern "C" int fkc_launch(fkc_ctx* c, int kernel, const void* params, size_t par
   }
   cudaSetDevice(c->device);
   return k.launch(c, p, bufs);
+}
+
+extern "C" int fkc_linear_mxfp4_work(uint32_t entries, uint32_t n, uint32_t kk, uint32_t m, uint32_t k,
+                                     size_t* bytes) {
+  if (!bytes) return fail(FKC_ERR_ARGUMENT, "fkc_linear_mxfp4_work: no place for the size.");
+  *bytes = fk_linear_mxfp4_work(entries, n, kk, m, k);
+  return FKC_OK;
 }
 
 // ---------------------------------------------------------------------------

@@ -83,6 +83,10 @@ def _bf16(name, access="read"):
     return Buffer(name, access, "bf16")
 
 
+def _u8(name, access="read"):
+    return Buffer(name, access, "u8")
+
+
 def _dim(name, lo, hi, mult=1):
     return Param(name, "u32", DimRange(lo, hi, mult))
 
@@ -192,6 +196,24 @@ SPEC_KERNELS = {
         KernelSig("gated_gelu", [_f32("x"), _f32("y", "write")], [_dim("segments", 1, _MAX), _dim("f", 1, _MAX)]),
         KernelSig("combine_ranks_add", [_f32("r"), _f32("ws"), _f32("segs"), _f32("y", "write")],
                   [_dim("m", 1, 65535), _dim("k", 1, 8), _dim("d", 1, _MAX)]),
+        # The grouped router, and MXFP4 weights (no counterpart in the
+        # reference's element types).
+        *[KernelSig(name, [_f32("x"), *bias, _u32("ids", "write"), _f32("ws", "write")],
+                    [_dim("m", 1, 1048576), _dim("n", 1, 1024), _dim("k", 1, 8), _dim("groups", 1, 32),
+                     _dim("top_groups", 1, 32), _dim("group_by", 1, 2), _dim("sigmoid", 0, 1), _dim("renorm", 0, 1),
+                     _u("ldx"), _f("factor")], threads=128)
+          for name, bias in (("route_grouped", []), ("route_grouped_bias", [_f32("bias")]))],
+        KernelSig("quant_mxfp4", [_f32("x"), _u8("codes", "write"), _u8("scales", "write")],
+                  [_dim("rows", 1, 268435456), _dim("k", 32, 1048576, 32), _u("ldx")]),
+        KernelSig("widen_mxfp4", [_u8("codes"), _u8("scales"), _f32("y", "write")],
+                  [_dim("rows", 1, 268435456), _dim("k", 32, 1048576, 32), _u("ldy")]),
+        KernelSig("linear_mxfp4", [_u8("w"), _u8("w_scale"), _f32("x"), _f32("y", "write"), _u8("work", "read_write")],
+                  [_dim("n", 1, 1048576), _dim("k", 32, 65536, 32), _dim("m", 1, 65535), _u("ldx"), _u("ldy")]),
+        KernelSig("linear_routed_mxfp4",
+                  [_u8("table"), _u8("t_scale"), _u32("ids"), _f32("x"), _f32("y", "write"),
+                   _u8("work", "read_write")],
+                  [_dim("entries", 1, 4096), _dim("n", 1, 1048576), _dim("kk", 32, 65536, 32), _dim("m", 1, 65535),
+                   _dim("k", 1, 8), _u("ldx"), _u("ldy"), _dim("per_rank", 0, 1)]),
         # Paged caches (Graph.hs:144-152): a row's block table (indices)
         # instead of its slot; each cache's blocks through a table of their
         # addresses (IR.hs:400-429), bound after the buffers.
@@ -231,6 +253,7 @@ SPEC_KERNELS = {
 # Graph.hs:169-180): an f32 entry's parameters with the named buffers of
 # that type, named by the suffix of the type.
 WEIGHT_SUFFIX = {"f32": "", "bf16": "_wbf16", "f16": "_wf16"}
+INPUT_SUFFIX = {"f32": "", "bf16": "_xbf16", "f16": "_xf16"}  # the activations' type: the router's and MXFP4's entries
 CACHE_SUFFIX = {"f32": "", "bf16": "_kvbf16", "f16": "_kvf16"}
 _VARIANTS = [
     *[(base, base + WEIGHT_SUFFIX[t], {"w", "gamma"}, t)
@@ -241,6 +264,11 @@ _VARIANTS = [
       for t in ("bf16", "f16")
       for base, buf in (("gather", "table"), ("rmsnorm_rows", "gamma"), ("split_tf32", "x"),
                         ("gemv_routed", "table"), ("route_topk_scaled", "scale"))],
+    *[(base, base + INPUT_SUFFIX[t], bufs, t)
+      for t in ("bf16", "f16")
+      for base, bufs in (("route_grouped", {"x"}), ("route_grouped_bias", {"x"}), ("quant_mxfp4", {"x"}),
+                         ("linear_mxfp4", {"x", "y"}), ("linear_routed_mxfp4", {"x", "y"}))],
+    *[("widen_mxfp4", "widen_mxfp4_y" + t, {"y"}, t) for t in ("bf16", "f16")],
     *[(base, base + CACHE_SUFFIX[t], {"k_cache", "v_cache"}, t)
       for t in ("bf16", "f16")
       for base in ("kv_store_ring", "attend_split", "attend_decode", "attend_prompt", "kv_store_paged",

@@ -173,6 +173,12 @@ uint64_t fkc_fnv1a64(const void *bytes, size_t n);
  * dimensions are checked against their ranges first. */
 int fkc_launch(fkc_ctx *ctx, int kernel, const void *params, size_t params_len, void *const *bufs, int nbufs);
 
+/* The bytes of the `work` buffer that linear_mxfp4 (entries 1, k 1) and
+ * linear_routed_mxfp4 take for these sizes, whatever their type:
+ * 5 m k kk + 16 min(m k, 512) n + 16 m k + 64 entries + 65536. The launch
+ * writes it before it reads it; what it holds between launches is nobody's. */
+int fkc_linear_mxfp4_work(uint32_t entries, uint32_t n, uint32_t kk, uint32_t m, uint32_t k, size_t *bytes);
+
 /* ---- the tree reduction without allocation --------------------------------- */
 /* No counterpart in the reference. The sum of n f32 values at x into *y, with
  * exactly the bits of the reduce_groups + reduce_final launches, for callers
