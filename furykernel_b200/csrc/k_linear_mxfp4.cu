@@ -103,11 +103,12 @@ size_t fk_linear_mxfp4_work(uint64_t entries, uint64_t n, uint64_t kk, uint64_t 
   return 5 * pairs * kk + 16 * (pairs < 512 ? pairs : 512) * n + 16 * pairs + 64 * entries + 65536;
 }
 
-cudaError_t fk_launch_linear_mxfp4(const FkLinearMx& a, FkElem e, bool pdl, cudaStream_t s) {
+cudaError_t fk_launch_linear_mxfp4(const FkLinearMx& a, FkElem e, int sms, int* err, bool pdl, cudaStream_t s) {
   if (a.m == 0 || a.n == 0) return cudaSuccess;
   if (a.kk == 0 || a.kk % fk::mx::kBlock != 0 || a.k == 0 || a.entries == 0 ||
       a.ldx < (uint64_t)a.kk * (a.per_rank ? a.k : 1) || a.ldy < (uint64_t)a.k * a.n)
     return cudaErrorInvalidValue;
+  if ((uint64_t)a.m * a.k > 8ull * a.entries) return fk_launch_linear_mxfp4_tile(a, e, sms, err, pdl, s);
   const dim3 grid((a.n + 7) / 8, a.entries);
 #define FK_CALL(E) fk_launch_ex(fk::lx::plain_kernel<E>, grid, dim3(256), 0, s, pdl, a)
   return FK_BY_ELEM(e, FK_CALL);

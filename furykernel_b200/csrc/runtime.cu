@@ -1051,7 +1051,7 @@ int linear_mxfp4(fkc_ctx* c, const FkLinearMx& a, FkElem el, const char* name) {
   if (a.ldy < yw)
     return fail(FKC_ERR_ARGUMENT, "%s: ldy %u is less than a row's %llu outputs.", name, a.ldy,
                 (unsigned long long)yw);
-  return launched(fk_launch_linear_mxfp4(a, el, c->pdl, c->stream), name);
+  return launched(fk_launch_linear_mxfp4(a, el, c->sms, c->status, c->pdl, c->stream), name);
 }
 // linear_mxfp4: w w_scale x y work | n k m ldx ldy
 template <FkElem EL>
