@@ -84,6 +84,37 @@ __device__ __forceinline__ void load8(const typename E::Storage* p, uint32_t i, 
   }
 }
 
+// How far to move a run of inputs so that binary16 holds them best: the
+// power of two that takes the largest finite magnitude (its bits) into
+// [2^14, 2^15), at most 2^127. Binary16 inputs stay as they are.
+template <class E>
+__device__ __forceinline__ int input_shift(uint32_t top) {
+  if (E::kElem == FK_F16 || top == 0) return 0;
+  return min(141 - (int)(top >> 23), 127);
+}
+
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
+  return b < 0x7F800000u ? b : 0u;
+}
+
+// Eight inputs times `by` as binary16 pairs, and what those leave (exact in
+// binary32; nothing of an infinity or a NaN) as binary16 pairs again.
+template <bool LOW>
+__device__ __forceinline__ void split8(const float (&v)[8], float by, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float s0 = __fmul_rn(v[2 * i], by), s1 = __fmul_rn(v[2 * i + 1], by);
+    const __half h0 = __float2half_rn(s0), h1 = __float2half_rn(s1);
+    hi[i] = (uint32_t)__half_as_ushort(h0) | (uint32_t)__half_as_ushort(h1) << 16;
+    if constexpr (LOW) {
+      const float l0 = isfinite(s0) ? __fsub_rn(s0, __half2float(h0)) : 0.0f;
+      const float l1 = isfinite(s1) ? __fsub_rn(s1, __half2float(h1)) : 0.0f;
+      lo[i] = (uint32_t)__half_as_ushort(__float2half_rn(l0)) | (uint32_t)__half_as_ushort(__float2half_rn(l1)) << 16;
+    }
+  }
+}
+
 // A binary32 result stored in the output's type: rounded once, to nearest.
 template <class E>
 __device__ __forceinline__ void store(typename E::Storage* p, float v) {

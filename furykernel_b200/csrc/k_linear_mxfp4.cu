@@ -1,101 +1,298 @@
 // Products with MXFP4 weights (fk_mxfp4.cuh): y[r, j] = W[ids[r, j]] x[r],
 // or x[r, j] where each rank has its own input; a dense product is one
 // expert that every row takes. x and y in f32, bf16 or f16; the products
-// and sums in binary32, the result rounded once.
+// and sums in binary32, the result rounded once. Two kernels: the streaming
+// one below for few rows an expert, the tcgen05 one
+// (k_linear_mxfp4_tile.cu) for more.
+//
+// The streaming kernel reads every weight once for up to R rows and is held
+// by HBM, so the arithmetic a weight has to be little: at 23 bytes (43
+// weights) a cycle an SM there are three instructions a weight. The codes
+// widen to binary16 two an instruction and go to the tensor cores' warp-wide
+// products (16 weight rows x 16 of K x 8 columns) unscaled; a block of 32
+// weights, two such products, is one scale, which multiplies the block's
+// sums. The columns are the inputs: a row as two binary16 parts, x = h1 +
+// h2 relative to the largest of the block's 32 (within 2^-23 of x or 2^-39
+// of that largest), so 8 columns are 4 rows. Sums of blocks are binary32.
 #include "fk_common.cuh"
 #include "fk_kernels.h"
 #include "fk_mxfp4.cuh"
 
 namespace fk {
-namespace lx {
+namespace ls {
 
-constexpr int kPairsAPass = 8;
-constexpr uint32_t kPairWindow = 1024;  // (row, rank) pairs a block lists at a time
+constexpr uint32_t kWarps = 16;
+constexpr uint32_t kThreads = 32 * kWarps;
+constexpr uint32_t kTileRows = 16;     // weight rows of a unit
+constexpr uint32_t kStageBlocks = 4;   // blocks of 32 weights a row a stage
+constexpr uint32_t kStages = 4;        // a warp's own ring
+constexpr uint32_t kPitch = 80;        // a row's 64 bytes of codes: rows 20 banks apart, no two of 8 alike
+constexpr uint32_t kStageBytes = kTileRows * (kPitch + 8);
+constexpr uint32_t kMaxPairs = 512;
+constexpr uint32_t kMaxEntries = 4096;
+constexpr uint32_t kInputBudget = 114 * 1024;  // the inputs of a pass: 4.125 bytes an element
 
-// The plain kernel: a block a (expert, 8 output rows), a warp a row. It
-// lists the (row, rank) pairs that chose its expert and takes up to 8 at a
-// time: a lane a block of 32 weights, its dot with each pair's inputs, then
-// the warp's sum.
-template <class E>
-__global__ void __launch_bounds__(256) plain_kernel(FkLinearMx a) {
-  __shared__ uint32_t pairs[kPairWindow];
-  __shared__ uint32_t npairs;
-  const uint32_t e = blockIdx.y;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  grid_wait();
-  grid_launch_dependents();
-  const uint32_t all = a.m * a.k;
-  const uint32_t o = blockIdx.x * 8u + (uint32_t)warp;
-  const uint32_t blocks = a.kk / mx::kBlock;
-  const size_t row = (size_t)e * a.n + (o < a.n ? o : 0);
-  const uint4* wr = reinterpret_cast<const uint4*>(a.w) + row * blocks;
-  const uint8_t* sr = a.scales + row * blocks;
-  const bool wide = (uint64_t)a.ldx * sizeof(typename E::Storage) % 16 == 0;
-  const typename E::Storage* x = static_cast<const typename E::Storage*>(a.x);
-  typename E::Storage* y = static_cast<typename E::Storage*>(a.y);
-  for (uint32_t w0 = 0; w0 < all; w0 += kPairWindow) {
-    const uint32_t w1 = min(all, w0 + kPairWindow);
-    __syncthreads();
-    if (warp == 0) {
-      uint32_t c = 0;
-      for (uint32_t base = w0; base < w1; base += 32u) {
-        const uint32_t p = base + (uint32_t)lane;
-        const bool hit = p < w1 && (!a.ids || a.ids[p] == e);
-        const uint32_t mask = __ballot_sync(0xffffffffu, hit);
-        if (hit) pairs[c + __popc(mask & ((1u << lane) - 1u))] = p;
-        c += __popc(mask);
-        // A pair without an expert: its segment is 0, written by expert 0's blocks.
-        if (a.ids && e == 0 && p < w1 && a.ids[p] >= a.entries)
-          for (uint32_t q = blockIdx.x * 8u; q < min(a.n, blockIdx.x * 8u + 8u); ++q)
-            mx::store<E>(y + (size_t)(p / a.k) * a.ldy + (size_t)(p % a.k) * a.n + q, 0.0f);
-      }
-      if (lane == 0) npairs = c;
-    }
-    __syncthreads();
-    const uint32_t P = npairs;
-    if (P == 0 || o >= a.n) continue;
-    for (uint32_t p0 = 0; p0 < P; p0 += kPairsAPass) {
-      const uint32_t np = min((uint32_t)kPairsAPass, P - p0);
-      float acc[kPairsAPass];
-#pragma unroll
-      for (int q = 0; q < kPairsAPass; ++q) acc[q] = 0.0f;
-      for (uint32_t b = lane; b < blocks; b += 32) {
-        const uint4 cw = __ldg(wr + b);
-        const float s = mx::scale_value(__ldg(sr + b));
-        const uint32_t words[4] = {cw.x, cw.y, cw.z, cw.w};
-        float dot[kPairsAPass];
-#pragma unroll
-        for (int q = 0; q < kPairsAPass; ++q) dot[q] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float wv[8];
-          mx::widen8(words[i], wv);
-#pragma unroll
-          for (int q = 0; q < kPairsAPass; ++q) {
-            if ((uint32_t)q >= np) continue;
-            const uint32_t pr = pairs[p0 + q], r = pr / a.k, j = pr % a.k;
-            float xv[8];
-            mx::load8<E>(x + (size_t)r * a.ldx + (a.per_rank ? (size_t)j * a.kk : 0), 32 * b + 8 * i, wide, xv);
-#pragma unroll
-            for (int t = 0; t < 8; ++t) dot[q] = fmaf(wv[t], xv[t], dot[q]);
-          }
-        }
-#pragma unroll
-        for (int q = 0; q < kPairsAPass; ++q) acc[q] = fmaf(dot[q], s, acc[q]);
-      }
-#pragma unroll
-      for (int q = 0; q < kPairsAPass; ++q) {
-        const float total = warp_sum(acc[q]);
-        if ((uint32_t)q < np && lane == 0) {
-          const uint32_t pr = pairs[p0 + q];
-          mx::store<E>(y + (size_t)(pr / a.k) * a.ldy + (size_t)(pr % a.k) * a.n + o, total);
-        }
-      }
-    }
-  }
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// Four bytes, of which `have` are there (the others become 0).
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, uint32_t have) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(have) : "memory");
+}
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-}  // namespace lx
+// A pass: up to R pairs of one expert, at `first` of the grouped pairs.
+struct Pass {
+  uint16_t first, count;
+  uint32_t e;
+};
+
+// Persistent blocks over units (pass, 16 weight rows), neighbouring units a
+// block. The 16 warps share a unit's K, each with a ring of its own, so that
+// a warp's loads run on over the units; a barrier a unit adds the warps'
+// sums.
+template <class E, int R>
+__global__ void __launch_bounds__(kThreads, 1) stream_kernel(const FkLinearMx a) {
+  constexpr int NT = (R + 3) / 4;  // products of 8 columns
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ Pass passes[kMaxPairs];
+  __shared__ uint16_t perm[kMaxPairs];
+  __shared__ uint32_t ids_s[kThreads];
+  __shared__ float red[2][kWarps][kTileRows * R];
+  __shared__ uint32_t sums[2][kWarps], npasses_s, nrest_s;
+  uint8_t* rings = smem;                                        // [kWarps][kStages][kStageBytes]
+  uint8_t* xs = rings + kWarps * kStages * kStageBytes;         // [blocks][R][4][2] 16 bytes
+  const uint32_t blocks = a.kk / mx::kBlock;
+  float* sxs = reinterpret_cast<float*>(xs + (size_t)blocks * R * 128);  // [blocks][R]
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const uint32_t pairs = a.m * a.k, tiles = (a.n + kTileRows - 1) / kTileRows;
+
+  // The weights too may be the previous launch's (quant_mxfp4's): nothing is read before it is done.
+  grid_wait();
+  grid_launch_dependents();
+  uint32_t npasses, rest = 0;
+  if (a.ids) {
+    // The pairs of each expert, in the input's space (not filled yet).
+    uint32_t* count = reinterpret_cast<uint32_t*>(xs);
+    const uint32_t most = (a.entries + kThreads - 1) / kThreads;  // experts a thread, at most 8
+    for (uint32_t e = tid; e < most * kThreads; e += kThreads) count[e] = 0;
+    // A pair's expert (entries: none) and its place among the expert's pairs,
+    // by index: every block has to list them alike.
+    const uint32_t own = tid < pairs ? min(__ldg(a.ids + tid), a.entries) : 0xffffffffu;
+    ids_s[tid] = own;
+    __syncthreads();
+    uint32_t place = 0;
+    if (own < a.entries) atomicAdd(&count[own], 1u);
+    for (uint32_t q = 0; q < (tid & ~31u) + 32 && q < pairs; ++q) place += q < tid && ids_s[q] == own;
+    __syncthreads();
+    uint32_t c[8], mine = 0, mypass = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+      c[j] = j < most ? count[tid * most + j] : 0u;
+      mine += c[j];
+      mypass += (c[j] + R - 1) / R;
+    }
+    uint32_t is = mine, ip = mypass;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xffffffffu, is, d), v = __shfl_up_sync(0xffffffffu, ip, d);
+      if (lane >= (uint32_t)d) is += u, ip += v;
+    }
+    if (lane == 31) sums[0][warp] = is, sums[1][warp] = ip;
+    __syncthreads();
+    uint32_t bs = 0, bp = 0;
+    for (uint32_t w = 0; w < warp; ++w) bs += sums[0][w], bp += sums[1][w];
+    uint32_t s = bs + is - mine, p = bp + ip - mypass;
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+      if (j >= most) break;
+      count[tid * most + j] = s;
+      for (uint32_t q = 0; q < c[j]; q += R) {
+        passes[p].first = (uint16_t)(s + q);
+        passes[p].count = (uint16_t)min((uint32_t)R, c[j] - q);
+        passes[p].e = tid * most + j;
+        ++p;
+      }
+      s += c[j];
+    }
+    if (tid == kThreads - 1) npasses_s = p, nrest_s = s;
+    __syncthreads();
+    npasses = npasses_s;
+    rest = nrest_s;
+    if (tid < pairs) perm[(own < a.entries ? count[own] : rest) + place] = (uint16_t)tid;
+    __syncthreads();
+    // Pairs without an expert: zeros.
+    for (uint32_t q = rest + blockIdx.x; q < pairs; q += gridDim.x)
+      for (uint32_t i = tid; i < a.n; i += kThreads)
+        mx::store<E>(static_cast<typename E::Storage*>(a.y) + (size_t)(perm[q] / a.k) * a.ldy +
+                         (size_t)(perm[q] % a.k) * a.n + i,
+                     0.0f);
+  } else {
+    npasses = (pairs + R - 1) / R;
+    if (tid < npasses) {
+      passes[tid].first = (uint16_t)(tid * R);
+      passes[tid].count = (uint16_t)min((uint32_t)R, pairs - tid * R);
+      passes[tid].e = 0;
+    }
+    if (tid < pairs) perm[tid] = (uint16_t)tid;
+    __syncthreads();
+  }
+
+  const uint64_t units = (uint64_t)npasses * tiles;
+  const uint32_t u0 = (uint32_t)(blockIdx.x * units / gridDim.x), u1 = (uint32_t)((blockIdx.x + 1) * units / gridDim.x);
+  // This warp's blocks of every row.
+  const uint32_t b0 = warp * blocks / kWarps, nb = (warp + 1) * blocks / kWarps - b0;
+  const uint32_t steps = (nb + kStageBlocks - 1) / kStageBlocks;
+  uint8_t* ring = rings + warp * kStages * kStageBytes;
+  const uint64_t scale_bytes = (uint64_t)a.entries * a.n * blocks;
+
+  // The loads of the next stage: the warp's own cursor over (unit, step).
+  uint32_t lu = u0, ls = 0, slot = 0;
+  auto load = [&]() {
+    if (lu < u1 && steps) {
+      const uint64_t row0 = (uint64_t)passes[lu / tiles].e * a.n;
+      const uint32_t r0 = (lu % tiles) * kTileRows, at = b0 + ls * kStageBlocks;
+      const uint32_t have = min(kStageBlocks, nb - ls * kStageBlocks);
+      uint8_t* st = ring + slot * kStageBytes;
+#pragma unroll
+      for (uint32_t i = 0; i < 2; ++i) {
+        const uint32_t row = (lane >> 2) + 8 * i, c = lane & 3;
+        if (c < have)
+          copy16(smem_at(st + row * kPitch + c * 16),
+                 a.w + ((row0 + min(r0 + row, a.n - 1)) * blocks + at + c) * 16);
+      }
+      // A row's scales: the words that hold their bytes, wherever they start.
+      const uint64_t first = (row0 + min(r0 + (lane >> 1), a.n - 1)) * blocks + at;
+      const uint64_t word = (first & ~3ull) + 4 * (lane & 1);
+      if (word < first + have)
+        copy4(smem_at(st + kTileRows * kPitch + lane * 4), a.scales + word,
+              (uint32_t)min((uint64_t)4, scale_bytes - word));
+      if (++ls == steps) ls = 0, ++lu;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    slot = slot + 1 == kStages ? 0 : slot + 1;
+  };
+#pragma unroll
+  for (uint32_t i = 0; i < kStages - 1; ++i) load();
+
+  uint32_t pass = 0xffffffffu, use = 0;
+  for (uint32_t u = u0; u < u1; ++u) {
+    if (u / tiles != pass) {
+      // The pass's inputs as parts, a thread 8 of them, 4 threads a block.
+      pass = u / tiles;
+      __syncthreads();
+      const Pass ps = passes[pass];
+      for (uint32_t i = tid; i < ps.count * blocks * 4; i += kThreads) {
+        const uint32_t r = i / (blocks * 4), b = i / 4 % blocks, q = i & 3;
+        const uint32_t p = perm[ps.first + r];
+        const typename E::Storage* x = static_cast<const typename E::Storage*>(a.x) + (size_t)(p / a.k) * a.ldx +
+                                       (a.per_rank ? (size_t)(p % a.k) * a.kk : 0);
+        float v[8];
+        mx::load8<E>(x, 32 * b + 8 * q, ((uintptr_t)x & 15) == 0, v);
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, mx::finite_bits(v[j]));
+        const uint32_t quad = 0xFu << (lane & 28u);  // the block's threads leave the loop together
+        top = max(top, __shfl_xor_sync(quad, top, 1));
+        top = max(top, __shfl_xor_sync(quad, top, 2));
+        const int up = mx::input_shift<E>(top);
+        uint32_t hi[4], lo[4];
+        mx::split8<true>(v, mx::scale_value((uint32_t)(127 + up)), hi, lo);
+        uint4* to = reinterpret_cast<uint4*>(xs) + ((b * R + r) * 4 + q) * 2;
+        to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        to[1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if (q == 0) sxs[b * R + r] = mx::scale_value((uint32_t)(127 - up));
+      }
+      __syncthreads();
+    }
+    const uint32_t rows = passes[pass].count;
+    const uint64_t row0 = (uint64_t)passes[pass].e * a.n;
+    const uint32_t r0 = (u % tiles) * kTileRows;
+    float acc[NT][2];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = 0.0f;
+    for (uint32_t step = 0; step < steps; ++step) {
+      load();
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+      __syncwarp();
+      const uint8_t* st = ring + use * kStageBytes;
+      use = use + 1 == kStages ? 0 : use + 1;
+      const uint32_t at = b0 + step * kStageBlocks, have = min(kStageBlocks, nb - step * kStageBlocks);
+      // The four scale bytes of rows g and g + 8, shifted to the word's start.
+      uint32_t sc[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint2 w = *reinterpret_cast<const uint2*>(st + kTileRows * kPitch + (g + 8 * h) * 8);
+        const uint32_t off = (uint32_t)((row0 + min(r0 + g + 8 * h, a.n - 1)) * blocks + at) & 3u;
+        sc[h] = __funnelshift_r(w.x, w.y, 8 * off);
+      }
+#pragma unroll
+      for (uint32_t b = 0; b < kStageBlocks; ++b) {
+        if (b >= have) break;
+        const uint32_t w0 = *reinterpret_cast<const uint32_t*>(st + g * kPitch + b * 16 + t * 4);
+        const uint32_t w1 = *reinterpret_cast<const uint32_t*>(st + (g + 8) * kPitch + b * 16 + t * 4);
+        uint32_t p[4], q[4];
+        mx::widen8_f16(w0, p);
+        mx::widen8_f16(w1, q);
+        const float s0 = mx::scale_value((sc[0] >> (8 * b)) & 0xFFu), s1 = mx::scale_value((sc[1] >> (8 * b)) & 0xFFu);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          uint4 x = make_uint4(0, 0, 0, 0);
+          const uint32_t r = 4 * j + (g >> 1);
+          if (r < rows)
+            x = reinterpret_cast<const uint4*>(xs)[(((at + b) * R + r) * 4 + t) * 2 + (g & 1)];
+          const float sx = sxs[(at + b) * R + min(4 * j + t, (uint32_t)R - 1)];
+          float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          mma(d, p[0], q[0], p[1], q[1], x.x, x.y);
+          mma(d, p[2], q[2], p[3], q[3], x.z, x.w);
+          acc[j][0] = fmaf(__fadd_rn(d[0], d[1]), __fmul_rn(s0, sx), acc[j][0]);
+          acc[j][1] = fmaf(__fadd_rn(d[2], d[3]), __fmul_rn(s1, sx), acc[j][1]);
+        }
+      }
+      __syncwarp();  // before the stage is loaded again
+    }
+    float(*rd)[kTileRows * R] = red[u & 1];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+      if (4 * j + t < (uint32_t)R) {
+        rd[warp][(4 * j + t) * kTileRows + g] = acc[j][0];
+        rd[warp][(4 * j + t) * kTileRows + g + 8] = acc[j][1];
+      }
+    __syncthreads();
+    if (tid < kTileRows * rows && r0 + tid % kTileRows < a.n) {
+      float v = 0.0f;
+#pragma unroll
+      for (uint32_t w = 0; w < kWarps; ++w) v = __fadd_rn(v, rd[w][tid]);
+      const uint32_t p = perm[passes[pass].first + tid / kTileRows];
+      mx::store<E>(static_cast<typename E::Storage*>(a.y) + (size_t)(p / a.k) * a.ldy + (size_t)(p % a.k) * a.n + r0 +
+                       tid % kTileRows,
+                   v);
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+template <class E, int R>
+cudaError_t launch(const FkLinearMx& a, int sms, bool pdl, cudaStream_t s) {
+  const uint64_t pairs = (uint64_t)a.m * a.k, tiles = (a.n + kTileRows - 1) / kTileRows;
+  const uint32_t blocks = a.kk / mx::kBlock;
+  size_t input = (size_t)blocks * R * 132;
+  if (a.ids && input < (a.entries + kThreads) * 4) input = (a.entries + kThreads) * 4;  // the count's space
+  const size_t smem = kWarps * kStages * kStageBytes + input;
+  cudaError_t e = fk_allow_smem(stream_kernel<E, R>, smem);
+  if (e != cudaSuccess) return e;
+  const uint64_t units = pairs * tiles;  // at most
+  return fk_launch_ex(stream_kernel<E, R>, dim3((uint32_t)(units < (uint64_t)sms ? units : (uint64_t)sms)),
+                      dim3(kThreads), smem, s, pdl, a);
+}
+
+}  // namespace ls
 }  // namespace fk
 
 size_t fk_linear_mxfp4_work(uint64_t entries, uint64_t n, uint64_t kk, uint64_t m, uint64_t k) {
@@ -105,12 +302,19 @@ size_t fk_linear_mxfp4_work(uint64_t entries, uint64_t n, uint64_t kk, uint64_t 
 
 cudaError_t fk_launch_linear_mxfp4(const FkLinearMx& a, FkElem e, int sms, int* err, bool pdl, cudaStream_t s) {
   if (a.m == 0 || a.n == 0) return cudaSuccess;
-  if (a.kk == 0 || a.kk % fk::mx::kBlock != 0 || a.k == 0 || a.entries == 0 ||
+  if (a.kk == 0 || a.kk % fk::mx::kBlock != 0 || a.k == 0 || a.entries == 0 || a.entries > fk::ls::kMaxEntries ||
       a.ldx < (uint64_t)a.kk * (a.per_rank ? a.k : 1) || a.ldy < (uint64_t)a.k * a.n)
     return cudaErrorInvalidValue;
-  if ((uint64_t)a.m * a.k > 8ull * a.entries) return fk_launch_linear_mxfp4_tile(a, e, sms, err, pdl, s);
-  const dim3 grid((a.n + 7) / 8, a.entries);
-#define FK_CALL(E) fk_launch_ex(fk::lx::plain_kernel<E>, grid, dim3(256), 0, s, pdl, a)
-  return FK_BY_ELEM(e, FK_CALL);
+  const uint64_t pairs = (uint64_t)a.m * a.k;
+  const uint64_t fit = fk::ls::kInputBudget / ((uint64_t)a.kk / 32 * 132);  // rows a pass can hold
+  if (pairs <= fk::ls::kMaxPairs && pairs <= 8ull * a.entries && fit >= 1) {
+#define FK_CALL(E)                                                                                        \
+  (pairs == 1 || fit < 2     ? fk::ls::launch<E, 1>(a, sms, pdl, s)                                       \
+   : pairs == 2 || fit < 4   ? fk::ls::launch<E, 2>(a, sms, pdl, s)                                       \
+   : pairs <= 4ull * a.entries || fit < 8 ? fk::ls::launch<E, 4>(a, sms, pdl, s)                          \
+                             : fk::ls::launch<E, 8>(a, sms, pdl, s))
+    return FK_BY_ELEM(e, FK_CALL);
 #undef FK_CALL
+  }
+  return fk_launch_linear_mxfp4_tile(a, e, sms, err, pdl, s);
 }

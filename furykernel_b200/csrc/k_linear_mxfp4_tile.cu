@@ -524,33 +524,17 @@ __global__ void __launch_bounds__(256) split_kernel(SplitArgs a) {
     for (int i = 0; i < 8; ++i) v[h][i] = 0.0f;
     if (c < a.kk) mx::load8<E>(x, c, wide, v[h]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t b = __float_as_uint(v[h][i]) & 0x7FFFFFFFu;
-      if (b < 0x7F800000u) top = max(top, b);
-    }
+    for (int i = 0; i < 8; ++i) top = max(top, mx::finite_bits(v[h][i]));
   }
   top = __reduce_max_sync(0xffffffffu, top);
-  // x 2^up in binary16: the largest in [2^14, 2^15). Binary16 inputs stay as they are.
-  int up = 0;
-  if (E::kElem != FK_F16 && top) up = min(141 - (int)(top >> 23), 127);
+  const int up = mx::input_shift<E>(top);
   const float by = mx::scale_value((uint32_t)(127 + up));
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const uint32_t c = run * kRun + 256 * h + 8 * lane;
     if (c >= a.kk) continue;
     uint32_t lo[4], hi[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float s0 = __fmul_rn(v[h][2 * i], by), s1 = __fmul_rn(v[h][2 * i + 1], by);
-      const __half h0 = __float2half_rn(s0), h1 = __float2half_rn(s1);
-      hi[i] = (uint32_t)__half_as_ushort(h0) | (uint32_t)__half_as_ushort(h1) << 16;
-      if constexpr (PARTS == 2) {
-        // What is left is exact in binary32; nothing is left of an infinity or a NaN.
-        const float l0 = isfinite(s0) ? __fsub_rn(s0, __half2float(h0)) : 0.0f;
-        const float l1 = isfinite(s1) ? __fsub_rn(s1, __half2float(h1)) : 0.0f;
-        lo[i] = (uint32_t)__half_as_ushort(__float2half_rn(l0)) | (uint32_t)__half_as_ushort(__float2half_rn(l1)) << 16;
-      }
-    }
+    mx::split8<PARTS == 2>(v[h], by, hi, lo);
     uint16_t* to = a.parts + (size_t)slot * a.kk + c;
     *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     if constexpr (PARTS == 2)

@@ -281,7 +281,7 @@ def held_to_experts(y, codes, scales, ids, x, t, per_rank):
 
 
 @pytest.mark.parametrize("entries,n,kk,m,k", [(1, 40, 64, 1, 1), (8, 130, 96, 1, 2), (64, 72, 352, 16, 4),
-                                              (8, 200, 1056, 33, 2), (16, 129, 544, 100, 8), (4, 260, 512, 300, 3)])
+                                              (8, 200, 1056, 33, 2), (40, 1500, 512, 60, 4), (16, 129, 544, 100, 8), (4, 260, 512, 300, 3)])
 @pytest.mark.parametrize("per_rank", [False, True])
 @pytest.mark.parametrize("t", TYPES)
 def test_routed(ctx, entries, n, kk, m, k, per_rank, t):
