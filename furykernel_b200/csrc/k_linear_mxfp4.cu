@@ -153,27 +153,35 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const FkLinearMx a)
   const uint64_t scale_bytes = (uint64_t)a.entries * a.n * blocks;
 
   // The loads of the next stage: the warp's own cursor over (unit, step).
-  uint32_t lu = u0, ls = 0, slot = 0;
+  // Addresses are formed once a unit and move on by a stage.
+  uint32_t left = u1 - u0, ltile = u0 % tiles, lpass = u0 / tiles, ls = 0, slot = 0;
+  const uint8_t *lc0 = nullptr, *lc1 = nullptr;
+  uint64_t lscale = 0;
+  const uint32_t to0 = (lane >> 2) * kPitch + (lane & 3) * 16, to_scale = kTileRows * kPitch + lane * 4;
   auto load = [&]() {
-    if (lu < u1 && steps) {
-      const uint64_t row0 = (uint64_t)passes[lu / tiles].e * a.n;
-      const uint32_t r0 = (lu % tiles) * kTileRows, at = b0 + ls * kStageBlocks;
-      const uint32_t have = min(kStageBlocks, nb - ls * kStageBlocks);
-      uint8_t* st = ring + slot * kStageBytes;
-#pragma unroll
-      for (uint32_t i = 0; i < 2; ++i) {
-        const uint32_t row = (lane >> 2) + 8 * i, c = lane & 3;
-        if (c < have)
-          copy16(smem_at(st + row * kPitch + c * 16),
-                 a.w + ((row0 + min(r0 + row, a.n - 1)) * blocks + at + c) * 16);
+    if (left && steps) {
+      if (ls == 0) {
+        const uint64_t row0 = (uint64_t)passes[lpass].e * a.n;
+        const uint32_t r0 = ltile * kTileRows;
+        lc0 = a.w + ((row0 + min(r0 + (lane >> 2), a.n - 1)) * blocks + b0 + (lane & 3)) * 16;
+        lc1 = a.w + ((row0 + min(r0 + (lane >> 2) + 8, a.n - 1)) * blocks + b0 + (lane & 3)) * 16;
+        lscale = (row0 + min(r0 + (lane >> 1), a.n - 1)) * blocks + b0;
+      }
+      const uint32_t have = nb - ls * kStageBlocks;  // 4 or more: the whole stage
+      const uint32_t st = smem_at(ring + slot * kStageBytes);
+      if ((lane & 3) < have) {
+        copy16(st + to0, lc0);
+        copy16(st + to0 + 8 * kPitch, lc1);
       }
       // A row's scales: the words that hold their bytes, wherever they start.
-      const uint64_t first = (row0 + min(r0 + (lane >> 1), a.n - 1)) * blocks + at;
-      const uint64_t word = (first & ~3ull) + 4 * (lane & 1);
-      if (word < first + have)
-        copy4(smem_at(st + kTileRows * kPitch + lane * 4), a.scales + word,
-              (uint32_t)min((uint64_t)4, scale_bytes - word));
-      if (++ls == steps) ls = 0, ++lu;
+      const uint64_t word = (lscale & ~3ull) + 4 * (lane & 1);
+      if (word < lscale + min(kStageBlocks, have))
+        copy4(st + to_scale, a.scales + word, (uint32_t)min((uint64_t)4, scale_bytes - word));
+      lc0 += kStageBlocks * 16, lc1 += kStageBlocks * 16, lscale += kStageBlocks;
+      if (++ls == steps) {
+        ls = 0, --left;
+        if (++ltile == tiles) ltile = 0, ++lpass;
+      }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     slot = slot + 1 == kStages ? 0 : slot + 1;
@@ -181,80 +189,100 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const FkLinearMx a)
 #pragma unroll
   for (uint32_t i = 0; i < kStages - 1; ++i) load();
 
-  uint32_t pass = 0xffffffffu, use = 0;
-  for (uint32_t u = u0; u < u1; ++u) {
-    if (u / tiles != pass) {
+  uint32_t use = 0, tile = u0 % tiles, pass = u0 / tiles;
+  for (uint32_t u = u0; u < u1; ++u, ++tile) {
+    if (tile == tiles) tile = 0, ++pass;
+    if (tile == 0 || u == u0) {
       // The pass's inputs as parts, a thread 8 of them, 4 threads a block.
-      pass = u / tiles;
       __syncthreads();
       const Pass ps = passes[pass];
-      for (uint32_t i = tid; i < ps.count * blocks * 4; i += kThreads) {
-        const uint32_t r = i / (blocks * 4), b = i / 4 % blocks, q = i & 3;
-        const uint32_t p = perm[ps.first + r];
-        const typename E::Storage* x = static_cast<const typename E::Storage*>(a.x) + (size_t)(p / a.k) * a.ldx +
-                                       (a.per_rank ? (size_t)(p % a.k) * a.kk : 0);
-        float v[8];
-        mx::load8<E>(x, 32 * b + 8 * q, ((uintptr_t)x & 15) == 0, v);
-        uint32_t top = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, mx::finite_bits(v[j]));
-        const uint32_t quad = 0xFu << (lane & 28u);  // the block's threads leave the loop together
-        top = max(top, __shfl_xor_sync(quad, top, 1));
-        top = max(top, __shfl_xor_sync(quad, top, 2));
-        const int up = mx::input_shift<E>(top);
-        uint32_t hi[4], lo[4];
-        mx::split8<true>(v, mx::scale_value((uint32_t)(127 + up)), hi, lo);
-        uint4* to = reinterpret_cast<uint4*>(xs) + ((b * R + r) * 4 + q) * 2;
-        to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        to[1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        if (q == 0) sxs[b * R + r] = mx::scale_value((uint32_t)(127 - up));
+      const uint32_t eighths = blocks * 4, abreast = max(1u, kThreads / eighths);  // rows at once
+      const uint32_t stride = abreast > 1 ? eighths : kThreads;
+      for (uint32_t r = tid / eighths < abreast ? (abreast > 1 ? tid / eighths : 0u) : ps.count; r < ps.count;
+           r += abreast) {
+        for (uint32_t i = abreast > 1 ? tid % eighths : tid; i < eighths; i += stride) {
+          const uint32_t b = i >> 2, q = i & 3;
+          const uint32_t p = perm[ps.first + r];
+          const typename E::Storage* x = static_cast<const typename E::Storage*>(a.x) + (size_t)(p / a.k) * a.ldx +
+                                         (a.per_rank ? (size_t)(p % a.k) * a.kk : 0);
+          float v[8];
+          mx::load8<E>(x, 32 * b + 8 * q, ((uintptr_t)x & 15) == 0, v);
+          uint32_t top = 0;
+  #pragma unroll
+          for (int j = 0; j < 8; ++j) top = max(top, mx::finite_bits(v[j]));
+          const uint32_t quad = 0xFu << (lane & 28u);  // the block's threads leave the loop together
+          top = max(top, __shfl_xor_sync(quad, top, 1));
+          top = max(top, __shfl_xor_sync(quad, top, 2));
+          const int up = mx::input_shift<E>(top);
+          uint32_t hi[4], lo[4];
+          mx::split8<true>(v, mx::scale_value((uint32_t)(127 + up)), hi, lo);
+          uint4* to = reinterpret_cast<uint4*>(xs) + ((b * R + r) * 4 + q) * 2;
+          to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          to[1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          if (q == 0) sxs[b * R + r] = mx::scale_value((uint32_t)(127 - up));
+        }
       }
       __syncthreads();
     }
     const uint32_t rows = passes[pass].count;
     const uint64_t row0 = (uint64_t)passes[pass].e * a.n;
-    const uint32_t r0 = (u % tiles) * kTileRows;
+    const uint32_t r0 = tile * kTileRows;
     float acc[NT][2];
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = 0.0f;
+    // Where rows g and g + 8 have their scales' bytes in their words: a
+    // stage moves on by whole words.
+    uint32_t shift[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      shift[h] = 8 * ((uint32_t)((row0 + min(r0 + g + 8 * h, a.n - 1)) * blocks + b0) & 3u);
+    const uint4* xat = reinterpret_cast<const uint4*>(xs) + ((b0 * R + (g >> 1)) * 4 + t) * 2 + (g & 1);
+    const float* sat = sxs + b0 * R + (t < (uint32_t)R ? t : 0);
+    // One block of 32: two products, their sums times the block's scales.
+    auto block = [&](const uint8_t* st, uint32_t b, float s0, float s1) {
+      uint32_t p[4], q[4];
+      mx::widen8_f16(*reinterpret_cast<const uint32_t*>(st + g * kPitch + b * 16 + t * 4), p);
+      mx::widen8_f16(*reinterpret_cast<const uint32_t*>(st + (g + 8) * kPitch + b * 16 + t * 4), q);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (4 * j + (g >> 1) < rows) x = xat[(b * R + 4 * j) * 8];
+        const float sx = sat[b * R + 4 * j];
+        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        mma(d, p[0], q[0], p[1], q[1], x.x, x.y);
+        mma(d, p[2], q[2], p[3], q[3], x.z, x.w);
+        acc[j][0] = fmaf(__fadd_rn(d[0], d[1]), __fmul_rn(s0, sx), acc[j][0]);
+        acc[j][1] = fmaf(__fadd_rn(d[2], d[3]), __fmul_rn(s1, sx), acc[j][1]);
+      }
+    };
     for (uint32_t step = 0; step < steps; ++step) {
       load();
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
       __syncwarp();
       const uint8_t* st = ring + use * kStageBytes;
       use = use + 1 == kStages ? 0 : use + 1;
-      const uint32_t at = b0 + step * kStageBlocks, have = min(kStageBlocks, nb - step * kStageBlocks);
-      // The four scale bytes of rows g and g + 8, shifted to the word's start.
-      uint32_t sc[2];
+      const uint32_t have = nb - step * kStageBlocks;
+      uint32_t sc[2];  // four scale bytes of each row
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint2 w = *reinterpret_cast<const uint2*>(st + kTileRows * kPitch + (g + 8 * h) * 8);
-        const uint32_t off = (uint32_t)((row0 + min(r0 + g + 8 * h, a.n - 1)) * blocks + at) & 3u;
-        sc[h] = __funnelshift_r(w.x, w.y, 8 * off);
+        sc[h] = __funnelshift_r(w.x, w.y, shift[h]);
       }
+      // Whole stages with scales of 2^-126 .. 2^127, nearly all: the bytes
+      // are the factors' exponents.
+      const uint32_t odd = __vcmpeq4(sc[0], 0) | __vcmpeq4(sc[1], 0) | __vcmpeq4(sc[0], 0xFFFFFFFFu) |
+                           __vcmpeq4(sc[1], 0xFFFFFFFFu);
+      if (have >= kStageBlocks && !__any_sync(0xffffffffu, odd)) {
 #pragma unroll
-      for (uint32_t b = 0; b < kStageBlocks; ++b) {
-        if (b >= have) break;
-        const uint32_t w0 = *reinterpret_cast<const uint32_t*>(st + g * kPitch + b * 16 + t * 4);
-        const uint32_t w1 = *reinterpret_cast<const uint32_t*>(st + (g + 8) * kPitch + b * 16 + t * 4);
-        uint32_t p[4], q[4];
-        mx::widen8_f16(w0, p);
-        mx::widen8_f16(w1, q);
-        const float s0 = mx::scale_value((sc[0] >> (8 * b)) & 0xFFu), s1 = mx::scale_value((sc[1] >> (8 * b)) & 0xFFu);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          uint4 x = make_uint4(0, 0, 0, 0);
-          const uint32_t r = 4 * j + (g >> 1);
-          if (r < rows)
-            x = reinterpret_cast<const uint4*>(xs)[(((at + b) * R + r) * 4 + t) * 2 + (g & 1)];
-          const float sx = sxs[(at + b) * R + min(4 * j + t, (uint32_t)R - 1)];
-          float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          mma(d, p[0], q[0], p[1], q[1], x.x, x.y);
-          mma(d, p[2], q[2], p[3], q[3], x.z, x.w);
-          acc[j][0] = fmaf(__fadd_rn(d[0], d[1]), __fmul_rn(s0, sx), acc[j][0]);
-          acc[j][1] = fmaf(__fadd_rn(d[2], d[3]), __fmul_rn(s1, sx), acc[j][1]);
-        }
+        for (uint32_t b = 0; b < kStageBlocks; ++b)
+          block(st, b, __uint_as_float((b < 3 ? sc[0] << (23 - 8 * b) : sc[0] >> 1) & 0x7F800000u),
+                __uint_as_float((b < 3 ? sc[1] << (23 - 8 * b) : sc[1] >> 1) & 0x7F800000u));
+      } else {
+#pragma unroll 1
+        for (uint32_t b = 0; b < min(have, kStageBlocks); ++b)
+          block(st, b, mx::scale_value((sc[0] >> (8 * b)) & 0xFFu), mx::scale_value((sc[1] >> (8 * b)) & 0xFFu));
       }
+      xat += kStageBlocks * R * 8, sat += kStageBlocks * R;
       __syncwarp();  // before the stage is loaded again
     }
     float(*rd)[kTileRows * R] = red[u & 1];
@@ -265,13 +293,13 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const FkLinearMx a)
         rd[warp][(4 * j + t) * kTileRows + g + 8] = acc[j][1];
       }
     __syncthreads();
-    if (tid < kTileRows * rows && r0 + tid % kTileRows < a.n) {
+    if (tid < kTileRows * rows && r0 + (tid & 15) < a.n) {
       float v = 0.0f;
 #pragma unroll
       for (uint32_t w = 0; w < kWarps; ++w) v = __fadd_rn(v, rd[w][tid]);
-      const uint32_t p = perm[passes[pass].first + tid / kTileRows];
+      const uint32_t p = perm[passes[pass].first + (tid >> 4)];
       mx::store<E>(static_cast<typename E::Storage*>(a.y) + (size_t)(p / a.k) * a.ldy + (size_t)(p % a.k) * a.n + r0 +
-                       tid % kTileRows,
+                       (tid & 15),
                    v);
     }
   }
