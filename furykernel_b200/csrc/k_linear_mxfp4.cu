@@ -5,43 +5,60 @@
 // one below for few rows an expert, the tcgen05 one
 // (k_linear_mxfp4_tile.cu) for more.
 //
-// The streaming kernel reads every weight once for up to R rows and is held
-// by HBM, so the arithmetic a weight has to be little: at 23 bytes (43
-// weights) a cycle an SM there are three instructions a weight. The codes
-// widen to binary16 two an instruction and go to the tensor cores' warp-wide
-// products (16 weight rows x 16 of K x 8 columns) unscaled; a block of 32
+// The streaming kernel reads every weight once for up to R rows and should
+// be held by HBM, so the arithmetic a weight has to be little: at 23 bytes
+// (43 weights) a cycle an SM there are three instructions a weight, and one
+// and a half of the integer pipe's, which also widens codes. The codes go,
+// widened two an instruction to binary16 and unscaled, to the tensor cores'
+// warp-wide products (16 weight rows x 16 of K x 8 columns); a block of 32
 // weights, two such products, is one scale, which multiplies the block's
 // sums. The columns are the inputs: a row as two binary16 parts, x = h1 +
-// h2 relative to the largest of a stage's 128 (within 2^-23 of x or 2^-39
+// h2 relative to the largest of a stage's 256 (within 2^-23 of x or 2^-39
 // of that largest), so 8 columns are 4 rows. Sums of blocks are binary32.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include "fk_common.cuh"
 #include "fk_kernels.h"
 #include "fk_mxfp4.cuh"
+#include "fk_tcgen05.cuh"
 
 namespace fk {
 namespace ls {
 
+using namespace tc;
+
 constexpr uint32_t kWarps = 16;
 constexpr uint32_t kThreads = 32 * kWarps;
 constexpr uint32_t kTileRows = 16;     // weight rows of a unit
-constexpr uint32_t kStageBlocks = 4;   // blocks of 32 weights a row a stage
-constexpr uint32_t kStages = 4;        // a warp's own ring
-constexpr uint32_t kPitch = 80;        // a row's 64 bytes of codes: rows 20 banks apart, no two of 8 alike
-constexpr uint32_t kStageBytes = kTileRows * (kPitch + 8);
+constexpr uint32_t kStageBlocks = 8;   // blocks of 32 weights a row a stage: 128 bytes of codes
+constexpr uint32_t kMaxStages = 4;     // a warp's own ring
+constexpr uint32_t kCodeBytes = kTileRows * kStageBlocks * 16;
+constexpr uint32_t kScaleWords = 3;    // the words that hold 8 bytes, wherever they start
 constexpr uint32_t kMaxPairs = 512;
 constexpr uint32_t kMaxEntries = 4096;
-constexpr uint32_t kInputBudget = 114 * 1024;  // the inputs of the warps' passes
+constexpr uint32_t kSmemBudget = 227 * 1024 - 1024;  // static and dynamic, less the alignment's slack
 
-// A warp's inputs: `blocks` blocks of R rows, 128 bytes each (two parts),
+enum { LS_TIMEOUT = 29 };  // a stage of codes never landed
+
+// A stage's scale words and their values as factors.
+constexpr uint32_t kScaleBytes = kTileRows * kScaleWords * 4;
+constexpr uint32_t kFactorBytes = kTileRows * kStageBlocks * 4;
+
+// A warp's inputs: `steps` stages of R rows, two parts of 512 bytes each,
 // and a factor a row and stage.
-__host__ __device__ constexpr uint32_t input_bytes(uint32_t blocks, uint32_t R) {
-  return blocks * R * 128 + ((blocks + kStageBlocks - 1) / kStageBlocks * R * 4 + 15) / 16 * 16;
+__host__ __device__ constexpr uint32_t input_bytes(uint32_t steps, uint32_t R) {
+  return steps * R * kStageBlocks * 128 + (steps * R * 4 + 15) / 16 * 16;
+}
+__host__ __device__ constexpr uint32_t warp_bytes(uint32_t steps, uint32_t R, uint32_t stages) {
+  return stages * (kCodeBytes + kScaleBytes) + kFactorBytes + input_bytes(steps, R);
+}
+// Units whose sums wait together.
+__host__ __device__ constexpr uint32_t batch_of(uint32_t R) { return R <= 4 ? 8 : 4; }
+__host__ __device__ constexpr uint32_t static_bytes(uint32_t R) {
+  return kMaxPairs * 12 + kThreads * 4 + batch_of(R) * kWarps * kTileRows * R * 4 + 1024 + kWarps * kMaxStages * 8;
 }
 
-__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 // Four bytes, of which `have` are there (the others become 0).
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src, uint32_t have) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(have) : "memory");
@@ -52,7 +69,6 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-
 // The same onto zeros.
 __device__ __forceinline__ void mma0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                      uint32_t b1) {
@@ -73,27 +89,35 @@ struct Pass {
 // its own part of the inputs, so that only the unit's last sum needs the
 // others.
 template <class E, int R>
-__global__ void __launch_bounds__(kThreads, 1) stream_kernel(const FkLinearMx a, uint32_t share) {
+__global__ void __launch_bounds__(kThreads, 1)
+    stream_kernel(const __grid_constant__ CUtensorMap tw, const FkLinearMx a, uint32_t share, uint32_t stages,
+                  long long wait_cycles, int* __restrict__ err) {
   constexpr int NT = (R + 3) / 4;  // products of 8 columns
-  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr uint32_t kBatch = batch_of(R);
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t landed[kWarps][kMaxStages];
   __shared__ Pass passes[kMaxPairs];
-  __shared__ uint16_t perm[kMaxPairs];
+  __shared__ uint32_t perm[kMaxPairs];  // a pair's row, its rank << 16
   __shared__ uint32_t ids_s[kThreads];
-  __shared__ float red[2][kWarps][kTileRows * R];
+  __shared__ float red[kBatch][kWarps][kTileRows * R];
   __shared__ uint32_t sums[2][kWarps], npasses_s, nrest_s;
-  uint8_t* rings = smem;                                        // [kWarps][kStages][kStageBytes]
-  uint8_t* inputs = rings + kWarps * kStages * kStageBytes;     // [kWarps] input_bytes
-  const uint32_t blocks = a.kk / mx::kBlock;
+  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const uint32_t blocks = a.kk / mx::kBlock, all_steps = (blocks + kStageBlocks - 1) / kStageBlocks;
+  const uint32_t most_steps = (all_steps + share - 1) / share;
+  // [kWarps][stages] codes, then a warp's scale words, factors and inputs.
+  uint8_t* rest_smem = smem + kWarps * stages * kCodeBytes;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const uint32_t pairs = a.m * a.k, tiles = (a.n + kTileRows - 1) / kTileRows;
 
   // The weights too may be the previous launch's (quant_mxfp4's): nothing is read before it is done.
+  if (tid < kWarps * kMaxStages) mbar_init(smem_u32(&landed[0][0] + tid), 1);
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   grid_wait();
   grid_launch_dependents();
   uint32_t npasses, rest = 0;
   if (a.ids) {
     // The pairs of each expert, in the input's space (not filled yet).
-    uint32_t* count = reinterpret_cast<uint32_t*>(inputs);
+    uint32_t* count = reinterpret_cast<uint32_t*>(rest_smem);
     const uint32_t most = (a.entries + kThreads - 1) / kThreads;  // experts a thread, at most 8
     for (uint32_t e = tid; e < most * kThreads; e += kThreads) count[e] = 0;
     // A pair's expert (entries: none) and its place among the expert's pairs,
@@ -139,13 +163,13 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const FkLinearMx a,
     __syncthreads();
     npasses = npasses_s;
     rest = nrest_s;
-    if (tid < pairs) perm[(own < a.entries ? count[own] : rest) + place] = (uint16_t)tid;
+    if (tid < pairs) perm[(own < a.entries ? count[own] : rest) + place] = tid / a.k | (tid % a.k) << 16;
     __syncthreads();
     // Pairs without an expert: zeros.
     for (uint32_t q = rest + blockIdx.x; q < pairs; q += gridDim.x)
       for (uint32_t i = tid; i < a.n; i += kThreads)
-        mx::store<E>(static_cast<typename E::Storage*>(a.y) + (size_t)(perm[q] / a.k) * a.ldy +
-                         (size_t)(perm[q] % a.k) * a.n + i,
+        mx::store<E>(static_cast<typename E::Storage*>(a.y) + (size_t)(perm[q] & 0xFFFFu) * a.ldy +
+                         (size_t)(perm[q] >> 16) * a.n + i,
                      0.0f);
   } else {
     npasses = (pairs + R - 1) / R;
@@ -154,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const FkLinearMx a,
       passes[tid].count = (uint16_t)min((uint32_t)R, pairs - tid * R);
       passes[tid].e = 0;
     }
-    if (tid < pairs) perm[tid] = (uint16_t)tid;
+    if (tid < pairs) perm[tid] = tid / a.k | (tid % a.k) << 16;
     __syncthreads();
   }
 
@@ -162,154 +186,175 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const FkLinearMx a,
   const uint64_t units = (uint64_t)npasses * tiles, groups = (uint64_t)gridDim.x * abreast,
                  gid = (uint64_t)blockIdx.x * abreast + group;
   const uint32_t u0 = (uint32_t)(gid * units / groups), u1 = (uint32_t)((gid + 1) * units / groups);
-  // This warp's blocks of every row.
-  const uint32_t b0 = part * blocks / share, nb = (part + 1) * blocks / share - b0;
-  const uint32_t steps = (nb + kStageBlocks - 1) / kStageBlocks;
-  const uint32_t ring = smem_at(rings + warp * kStages * kStageBytes);
+  // This warp's stages of every row.
+  const uint32_t s0 = part * all_steps / share, steps = (part + 1) * all_steps / share - s0;
   const uint64_t scale_bytes = (uint64_t)a.entries * a.n * blocks;
+  const uint32_t ring = smem_u32(smem) + warp * stages * kCodeBytes;
+  uint8_t* mine_smem = rest_smem + warp * (warp_bytes(most_steps, R, stages) - stages * kCodeBytes);
+  const uint32_t scale_ring = smem_u32(mine_smem);
+  float* factors = reinterpret_cast<float*>(mine_smem + stages * kScaleBytes);  // [16 rows][8]
   // The inputs, [blocks][R][4][2] 16 bytes as the products take them, and
-  // the factors [steps][R].
-  const uint32_t most_blocks = (blocks + share - 1) / share;
-  uint8_t* xs = inputs + warp * input_bytes(most_blocks, R);
-  float* sxs = reinterpret_cast<float*>(xs + most_blocks * R * 128);
+  // the factors back, [steps][R].
+  uint8_t* xs = reinterpret_cast<uint8_t*>(factors) + kFactorBytes;
+  float* sxs = reinterpret_cast<float*>(xs + most_steps * kStageBlocks * R * 128);
 
   // The loads of the next stage: the warp's own cursor over (unit, step).
-  // Addresses are formed once a unit and move on by a stage.
-  uint32_t left = steps ? u1 - u0 : 0, ltile = u0 % tiles, lpass = u0 / tiles, ls = 0, lslot = 0;
-  const uint8_t *lc0 = nullptr, *lc1 = nullptr, *lsc = nullptr;
-  uint32_t loff = 0, lrest = 0;
-  const uint32_t to0 = (lane >> 2) * kPitch + (lane & 3) * 16, to_scale = kTileRows * kPitch + lane * 4;
+  // A unit's rows end with the table's: the last unit starts early enough
+  // (its first rows are another's too, with the same results).
+  uint32_t left = steps ? u1 - u0 : 0, ltile = u0 % tiles, lpass = u0 / tiles, ls = 0, lslot = 0, issued = 0;
+  const uint8_t* lsc = nullptr;
+  uint32_t lrest = 0, lrow = 0, lentry = 0;
+  int lword = 0;  // where the lane's word starts against its row's first byte
   auto load = [&]() {
     if (left) {
       if (ls == 0) {
-        const uint64_t row0 = (uint64_t)passes[lpass].e * a.n;
-        const uint32_t r0 = ltile * kTileRows;
-        lc0 = a.w + ((row0 + min(r0 + (lane >> 2), a.n - 1)) * blocks + b0 + (lane & 3)) * 16;
-        lc1 = a.w + ((row0 + min(r0 + (lane >> 2) + 8, a.n - 1)) * blocks + b0 + (lane & 3)) * 16;
-        // A row's scales: the words that hold their bytes, wherever they
-        // start; the table's last word may be short.
-        const uint64_t first = (row0 + min(r0 + (lane >> 1), a.n - 1)) * blocks + b0;
+        lentry = passes[lpass].e;
+        lrow = min(ltile * kTileRows, a.n - kTileRows);
+        const uint64_t first = ((uint64_t)lentry * a.n + lrow + (lane >> 1)) * blocks + s0 * kStageBlocks;
+        lword = (int)(4 * (lane & 1)) - (int)(first & 3);
         const uint64_t word = (first & ~3ull) + 4 * (lane & 1);
-        loff = 4 * (lane & 1) - (uint32_t)(first & 3);  // where the word starts against the first byte
         lsc = a.scales + word;
-        lrest = word < scale_bytes ? (uint32_t)min(scale_bytes - word, (uint64_t)0x40000000u) : 0u;
+        lrest = (uint32_t)min(scale_bytes - min(word, scale_bytes), (uint64_t)0x40000000u);
       }
-      const uint32_t have = min(nb - ls * kStageBlocks, kStageBlocks), st = ring + lslot;
-      if ((lane & 3) < have) {
-        copy16(st + to0, lc0);
-        copy16(st + to0 + 8 * kPitch, lc1);
+      if (lane == 0) {
+        const uint32_t bar = smem_u32(&landed[warp][lslot]);
+        mbar_expect_tx(bar, kCodeBytes);
+        tma_load_3d(ring + lslot * kCodeBytes, &tw, (int)((s0 + ls) * kStageBlocks * 16), (int)lrow, (int)lentry, bar);
       }
-      if ((int)loff < (int)have) copy4(st + to_scale, lsc, min(4u, lrest));
-      lc0 += kStageBlocks * 16, lc1 += kStageBlocks * 16, lsc += kStageBlocks, lrest -= kStageBlocks;
+      // Words 0 and 1 of a row, and the third where its bytes reach into it
+      // (the even lanes); the table's last word may be short.
+      const int have = (int)min(blocks - (s0 + ls) * kStageBlocks, kStageBlocks);
+      const uint32_t to = scale_ring + lslot * kScaleBytes + (lane >> 1) * kScaleWords * 4;
+      if (lword < have) copy4(to + (lane & 1) * 4, lsc, min(4u, lrest));
+      if (!(lane & 1) && lword + 8 < have) copy4(to + 8, lsc + 8, min(4u, lrest - 8));
+      lsc += kStageBlocks, lrest -= kStageBlocks;
+      ++issued;
       if (++ls == steps) {
         ls = 0, --left;
         if (++ltile == tiles) ltile = 0, ++lpass;
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-    lslot = lslot == (kStages - 1) * kStageBytes ? 0 : lslot + kStageBytes;
+    lslot = lslot + 1 == stages ? 0 : lslot + 1;
   };
-#pragma unroll
-  for (uint32_t i = 0; i < kStages - 1; ++i) load();
+  __syncthreads();  // the barriers are ready
+  for (uint32_t i = 0; i < stages - 1; ++i) load();
 
-  uint32_t slot = 0, tile = u0 % tiles, pass = u0 / tiles;
+  uint32_t slot = 0, phase = 0, held = 0, tile = u0 % tiles, pass = u0 / tiles;
+  bool lost = false;
+  auto group_sync = [&]() {
+    if (share > 1)
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * share) : "memory");
+    else
+      __syncwarp();
+  };
   for (uint32_t u = u0; u < u1; ++u, ++tile) {
     if (tile == tiles) tile = 0, ++pass;
     const Pass ps = passes[pass];
     if (tile == 0 || u == u0) {
-      // The warp's part of the pass's inputs: 16 lanes a row and stage, 8
-      // inputs a lane.
+      // The warp's part of the pass's inputs: a row and stage at a time, 8
+      // inputs a lane; zeros past the row's end.
       __syncwarp();
-      for (uint32_t i = lane >> 4; i < ps.count * steps; i += 2) {
-        const uint32_t r = i / steps, step = i - r * steps, c = step * kStageBlocks + ((lane >> 2) & 3), q = lane & 3;
+      for (uint32_t r = 0; r < ps.count; ++r) {
         const uint32_t p = perm[ps.first + r];
-        const typename E::Storage* x = static_cast<const typename E::Storage*>(a.x) + (size_t)(p / a.k) * a.ldx +
-                                       (a.per_rank ? (size_t)(p % a.k) * a.kk : 0);
-        float v[8];
+        const typename E::Storage* x = static_cast<const typename E::Storage*>(a.x) + (size_t)(p & 0xFFFFu) * a.ldx +
+                                       (a.per_rank ? (size_t)(p >> 16) * a.kk : 0);
+        const bool wide = ((uintptr_t)x & 15) == 0;
+#pragma unroll 2
+        for (uint32_t step = 0; step < steps; ++step) {
+          const uint32_t c = step * kStageBlocks + (lane >> 2), q = lane & 3;
+          float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-        if (c < nb) mx::load8<E>(x, 32 * (b0 + c) + 8 * q, ((uintptr_t)x & 15) == 0, v);
-        uint32_t top = 0;
+          for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+          if (s0 * kStageBlocks + c < blocks) mx::load8<E>(x, 32 * (s0 * kStageBlocks + c) + 8 * q, wide, v);
+          uint32_t top = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, mx::finite_bits(v[j]));
-        const uint32_t mask = 0xFFFFu << (lane & 16u);  // the stage's lanes leave the loop together
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(mask, top, o));
-        const int up = mx::input_shift<E>(top);
-        uint32_t hi[4], lo[4];
-        mx::split8<true>(v, mx::scale_value((uint32_t)(127 + up)), hi, lo);
-        if (c < nb) {
+          for (int j = 0; j < 8; ++j) top = max(top, mx::finite_bits(v[j]));
+          const int up = mx::input_shift<E>(__reduce_max_sync(0xffffffffu, top));
+          uint32_t hi[4], lo[4];
+          mx::split8<true>(v, mx::scale_value((uint32_t)(127 + up)), hi, lo);
           uint4* to = reinterpret_cast<uint4*>(xs) + ((c * R + r) * 4 + q) * 2;
           to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
           to[1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          if (lane == 0) sxs[step * R + r] = mx::scale_value((uint32_t)(127 - up));
         }
-        if ((lane & 15) == 0) sxs[step * R + r] = mx::scale_value((uint32_t)(127 - up));
       }
       __syncwarp();
     }
-    const uint64_t row0 = (uint64_t)ps.e * a.n;
-    const uint32_t r0 = tile * kTileRows;
+    const uint32_t r0 = min(tile * kTileRows, a.n - kTileRows);
+    // Where the scale bytes of row lane / 2 lie in their words (a stage moves on by whole words).
+    const uint32_t shift =
+        8 * ((uint32_t)(((uint64_t)ps.e * a.n + r0 + (lane >> 1)) * blocks + s0 * kStageBlocks) & 3u);
     float acc[NT][2];
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = 0.0f;
-    // Where rows g and g + 8 have their scales' bytes in their words: a
-    // stage moves on by whole words.
-    uint32_t shift[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      shift[h] = 8 * ((uint32_t)((row0 + min(r0 + g + 8 * h, a.n - 1)) * blocks + b0) & 3u);
     // Columns without a row take another's (R < 4) or what is there: each
     // column is its own, and theirs are not stored.
     const uint4* xat = reinterpret_cast<const uint4*>(xs) + (((g >> 1) % R) * 4 + t) * 2 + (g & 1);
     const float* sat = sxs + t % R;
     for (uint32_t step = 0; step < steps; ++step) {
       load();
-      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-      __syncwarp();
-      const uint8_t* st = rings + warp * kStages * kStageBytes + slot;
-      slot = slot == (kStages - 1) * kStageBytes ? 0 : slot + kStageBytes;
-      const uint32_t have = min(nb - step * kStageBlocks, kStageBlocks);
-      uint32_t sc[2];  // four scale bytes of each row
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint2 w = *reinterpret_cast<const uint2*>(st + kTileRows * kPitch + (g + 8 * h) * 8);
-        sc[h] = __funnelshift_r(w.x, w.y, shift[h]);
+      // All groups but the last stages - 1 have landed.
+      if (stages == 4)
+        asm volatile("cp.async.wait_group 3;" ::: "memory");
+      else if (stages == 3)
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+      else
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+      if (!lost && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&landed[warp][slot]), phase, wait_cycles))) {
+        lost = true;  // the results are not to be used: the status says so
+        if (lane == 0) record(err, LS_TIMEOUT);
       }
+      __syncwarp();
+      // The stage's scales as factors, four blocks of one row a lane: a byte
+      // is its factor's exponent, 0 is 2^-127 and infinity stands for NaN.
+      {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(mine_smem + slot * kScaleBytes) +
+                            (lane >> 1) * kScaleWords + (lane & 1);
+        uint32_t bytes = __funnelshift_r(w[0], w[1], shift);
+        const uint32_t have = blocks - (s0 + step) * kStageBlocks;
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float v = fmaxf(__uint_as_float((j < 3 ? bytes << (23 - 8 * j) : bytes >> 1) & 0x7F800000u),
+                                __uint_as_float(0x00400000u));
+          f[j] = fmaf(v, 0.0f, v);
+        }
+        if (have < kStageBlocks) {  // the row ends in this stage: no factor past it
+#pragma unroll
+          for (uint32_t j = 0; j < 4; ++j)
+            if (4 * (lane & 1) + j >= have) f[j] = 0.0f;
+        }
+        reinterpret_cast<float4*>(factors)[lane] = make_float4(f[0], f[1], f[2], f[3]);
+      }
+      __syncwarp();
+      const uint8_t* st = smem + (warp * stages + slot) * kCodeBytes + g * 128 + t * 4;
+      const float4* fg = reinterpret_cast<const float4*>(factors) + 2 * g;
       float sum[NT][2];
 #pragma unroll
       for (int j = 0; j < NT; ++j) sum[j][0] = sum[j][1] = 0.0f;
-      // One block of 32: two products, their sums times the block's scales.
-      auto block = [&](uint32_t b, float s0, float s1) {
-        uint32_t p[4], q[4];
-        mx::widen8_f16(*reinterpret_cast<const uint32_t*>(st + g * kPitch + b * 16 + t * 4), p);
-        mx::widen8_f16(*reinterpret_cast<const uint32_t*>(st + (g + 8) * kPitch + b * 16 + t * 4), q);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const uint4 x = xat[(b * R + 4 * j) * 8];
-          float d[4];
-          mma0(d, p[0], q[0], p[1], q[1], x.x, x.y);
-          mma(d, p[2], q[2], p[3], q[3], x.z, x.w);
-          sum[j][0] = fmaf(__fadd_rn(d[0], d[1]), s0, sum[j][0]);
-          sum[j][1] = fmaf(__fadd_rn(d[2], d[3]), s1, sum[j][1]);
+      for (uint32_t b4 = 0; b4 < kStageBlocks; b4 += 4) {
+        const float4 f0 = fg[b4 / 4], f1 = fg[16 + b4 / 4];
+        const float s0v[4] = {f0.x, f0.y, f0.z, f0.w}, s1v[4] = {f1.x, f1.y, f1.z, f1.w};
+#pragma unroll
+        for (uint32_t bb = 0; bb < 4; ++bb) {
+          // One block of 32: two products, their sums times the block's factors.
+          const uint32_t b = b4 + bb;
+          const uint8_t* at = st + ((b ^ g) << 4);  // the 128-byte swizzle
+          uint32_t p[4], q[4];
+          mx::widen8_f16(*reinterpret_cast<const uint32_t*>(at), p);
+          mx::widen8_f16(*reinterpret_cast<const uint32_t*>(at + 8 * 128), q);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const uint4 x = xat[(b * R + 4 * j) * 8];
+            float d[4];
+            mma0(d, p[0], q[0], p[1], q[1], x.x, x.y);
+            mma(d, p[2], q[2], p[3], q[3], x.z, x.w);
+            sum[j][0] = fmaf(__fadd_rn(d[0], d[1]), s0v[bb], sum[j][0]);
+            sum[j][1] = fmaf(__fadd_rn(d[2], d[3]), s1v[bb], sum[j][1]);
+          }
         }
-      };
-      // Scales of 2^-126 .. 2^127, nearly all: a byte is its factor's exponent.
-      auto plain = [&](uint32_t b, uint32_t w) {
-        return __uint_as_float((b < 3 ? w << (23 - 8 * b) : w >> 1) & 0x7F800000u);
-      };
-      const uint32_t odd = __vcmpeq4(sc[0], 0) | __vcmpeq4(sc[1], 0) | __vcmpeq4(sc[0], 0xFFFFFFFFu) |
-                           __vcmpeq4(sc[1], 0xFFFFFFFFu);
-      if (__any_sync(0xffffffffu, odd)) {
-#pragma unroll 1
-        for (uint32_t b = 0; b < have; ++b)
-          block(b, mx::scale_value((sc[0] >> (8 * b)) & 0xFFu), mx::scale_value((sc[1] >> (8 * b)) & 0xFFu));
-      } else if (have == kStageBlocks) {
-#pragma unroll
-        for (uint32_t b = 0; b < kStageBlocks; ++b) block(b, plain(b, sc[0]), plain(b, sc[1]));
-      } else {
-#pragma unroll
-        for (uint32_t b = 0; b < kStageBlocks - 1; ++b)
-          if (b < have) block(b, plain(b, sc[0]), plain(b, sc[1]));
       }
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
@@ -318,57 +363,101 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const FkLinearMx a,
         acc[j][1] = fmaf(sum[j][1], sx, acc[j][1]);
       }
       xat += kStageBlocks * R * 8, sat += R;
+      if (++slot == stages) slot = 0, phase ^= 1;
       __syncwarp();  // before the stage is loaded again
     }
-    float(*rd)[kTileRows * R] = red[u & 1];
+    // The warps' sums of up to kBatch units are added together at once: a
+    // barrier a unit, and the adding behind it, held the warps up for as
+    // long as half a unit's products.
+    float(*rd)[kTileRows * R] = red[held];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
       if (4 * j + t < (uint32_t)R) {
         rd[warp][(4 * j + t) * kTileRows + g] = acc[j][0];
         rd[warp][(4 * j + t) * kTileRows + g + 8] = acc[j][1];
       }
-    if (share > 1)
-      asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * share) : "memory");
-    else
-      __syncwarp();
-    for (uint32_t i = part * 32 + lane; i < kTileRows * ps.count; i += 32 * share) {
-      if (r0 + (i & 15) >= a.n) continue;
-      float v = 0.0f;
-      for (uint32_t w = 0; w < share; ++w) v = __fadd_rn(v, rd[group * share + w][i]);
-      const uint32_t p = perm[ps.first + (i >> 4)];
-      mx::store<E>(static_cast<typename E::Storage*>(a.y) + (size_t)(p / a.k) * a.ldy + (size_t)(p % a.k) * a.n + r0 +
-                       (i & 15),
+    if (++held < kBatch && u + 1 < u1) continue;
+    group_sync();
+    for (uint32_t o = part * 32 + lane; o < held * (kTileRows * R); o += 32 * share) {
+      const uint32_t uo = u + 1 - held + o / (kTileRows * R), i = o % (kTileRows * R);
+      const Pass po = passes[uo / tiles];
+      if ((i >> 4) >= po.count) continue;
+      const float* from = &red[o / (kTileRows * R)][group * share][i];
+      float v = from[0];
+#pragma unroll 4
+      for (uint32_t w = 1; w < share; ++w) v = __fadd_rn(v, from[w * (kTileRows * R)]);
+      const uint32_t p = perm[po.first + (i >> 4)];
+      mx::store<E>(static_cast<typename E::Storage*>(a.y) + (size_t)(p & 0xFFFFu) * a.ldy + (size_t)(p >> 16) * a.n +
+                       min(uo % tiles * kTileRows, a.n - kTileRows) + (i & 15),
                    v);
     }
+    held = 0;
+    group_sync();
   }
+  // Every stage issued was waited for above, so none is in flight (unless
+  // one was lost: then what is still out is waited for here, within limits).
   asm volatile("cp.async.wait_all;" ::: "memory");
+  if (lost)
+    for (uint32_t i = issued > stages ? issued - stages : 0; i < issued; ++i)
+      mbar_wait(smem_u32(&landed[warp][i % stages]), (i / stages) & 1, wait_cycles);
 }
 
-// How many warps share a unit: the fewest rounds of units, each its blocks
-// a warp and about 3 blocks' worth of fixed cost, and whose inputs fit.
-inline uint32_t share_of(uint64_t units, uint32_t blocks, uint32_t R, int sms) {
-  uint32_t best = 0;
+// How many warps share a unit, and how many stages a warp's ring has.
+struct Plan {
+  uint32_t share, stages;
+};
+
+// The fewest rounds of units, each its blocks a warp and about 4 blocks'
+// worth of fixed cost, whose inputs fit beside two stages a warp or more.
+inline Plan plan_of(uint64_t units, uint32_t blocks, uint32_t R, int sms) {
+  Plan best = {0, 0};
   uint64_t least = ~0ull;
+  const uint32_t all = (blocks + kStageBlocks - 1) / kStageBlocks;
   for (uint32_t share = kWarps; share >= 1; share /= 2) {
-    const uint32_t mine = (blocks + share - 1) / share;
-    const uint64_t at_once = (uint64_t)sms * (kWarps / share), cost = (units + at_once - 1) / at_once * (mine + 3);
-    if ((uint64_t)kWarps * input_bytes(mine, R) <= kInputBudget && cost < least) least = cost, best = share;
+    const uint32_t steps = (all + share - 1) / share;
+    const uint64_t at_once = (uint64_t)sms * (kWarps / share);
+    const uint64_t cost = (units + at_once - 1) / at_once * (steps * kStageBlocks + 4);
+    uint32_t stages = kMaxStages;
+    while (stages >= 2 && static_bytes(R) + (uint64_t)kWarps * warp_bytes(steps, R, stages) > kSmemBudget) --stages;
+    if (stages >= 2 && cost < least) least = cost, best = {share, stages};
   }
   return best;
 }
 
+// [entries][n][kk / 2] bytes of codes as boxes of 128 bytes x 16 rows,
+// 128-byte swizzle; zeros past a row's end.
+inline bool code_map(CUtensorMap* map, const FkLinearMx& a) {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  if (!fn) {
+    cudaDriverEntryPointQueryResult q;
+    void* p = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return false;
+    fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }
+  cuuint64_t dims[3] = {a.kk / 2, a.n, a.entries};
+  cuuint64_t strides[2] = {a.kk / 2, (cuuint64_t)a.kk / 2 * a.n};
+  cuuint32_t box[3] = {128, kTileRows, 1}, estr[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(a.w), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <class E, int R>
-cudaError_t launch(const FkLinearMx& a, uint32_t share, int sms, bool pdl, cudaStream_t s) {
+cudaError_t launch(const FkLinearMx& a, Plan plan, int sms, int* err, bool pdl, cudaStream_t s) {
   const uint64_t pairs = (uint64_t)a.m * a.k, tiles = (a.n + kTileRows - 1) / kTileRows;
-  const uint32_t blocks = a.kk / mx::kBlock;
-  size_t input = (size_t)kWarps * input_bytes((blocks + share - 1) / share, R);
-  if (a.ids && input < (a.entries + kThreads) * 4) input = (a.entries + kThreads) * 4;  // the count's space
-  const size_t smem = kWarps * kStages * kStageBytes + input;
+  const uint32_t all = (a.kk / mx::kBlock + kStageBlocks - 1) / kStageBlocks, share = plan.share;
+  size_t rest = (size_t)kWarps * (warp_bytes((all + share - 1) / share, R, plan.stages) - plan.stages * kCodeBytes);
+  if (a.ids && rest < (a.entries + kThreads) * 4) rest = (a.entries + kThreads) * 4;  // the count's space
+  const size_t smem = 1024 + (size_t)kWarps * plan.stages * kCodeBytes + rest;
+  CUtensorMap tw;
+  if (!code_map(&tw, a)) return cudaErrorInvalidValue;
   cudaError_t e = fk_allow_smem(stream_kernel<E, R>, smem);
   if (e != cudaSuccess) return e;
   const uint64_t most = (pairs * tiles + kWarps / share - 1) / (kWarps / share);  // blocks that have a unit
   return fk_launch_ex(stream_kernel<E, R>, dim3((uint32_t)(most < (uint64_t)sms ? most : (uint64_t)sms)),
-                      dim3(kThreads), smem, s, pdl, a, share);
+                      dim3(kThreads), smem, s, pdl, tw, a, share, plan.stages, (long long)4000000000LL, err);
 }
 
 }  // namespace ls
@@ -385,22 +474,23 @@ cudaError_t fk_launch_linear_mxfp4(const FkLinearMx& a, FkElem e, int sms, int* 
       a.ldx < (uint64_t)a.kk * (a.per_rank ? a.k : 1) || a.ldy < (uint64_t)a.k * a.n)
     return cudaErrorInvalidValue;
   const uint64_t pairs = (uint64_t)a.m * a.k;
-  if (pairs <= fk::ls::kMaxPairs && pairs <= 8ull * a.entries) {
+  if (pairs <= fk::ls::kMaxPairs && pairs <= 8ull * a.entries && a.n >= fk::ls::kTileRows) {
     // Rows a pass: 4 where an expert has that many on average, 8 past it,
     // fewer where there are no more or where they do not fit.
-    uint32_t R = pairs <= 2 ? (uint32_t)pairs : pairs <= 4ull * a.entries ? 4 : 8, share = 0;
+    uint32_t R = pairs <= 2 ? (uint32_t)pairs : pairs <= 4ull * a.entries ? 4 : 8;
+    fk::ls::Plan plan = {0, 0};
     const uint64_t experts = a.ids && pairs > a.entries ? a.entries : a.ids ? pairs : 1;  // at most
     for (; R >= 1; R /= 2) {
       const uint64_t passes = a.ids ? experts : (pairs + R - 1) / R;
-      share = fk::ls::share_of(passes * ((a.n + fk::ls::kTileRows - 1) / fk::ls::kTileRows), a.kk / 32, R, sms);
-      if (share) break;
+      plan = fk::ls::plan_of(passes * ((a.n + fk::ls::kTileRows - 1) / fk::ls::kTileRows), a.kk / 32, R, sms);
+      if (plan.share) break;
     }
-#define FK_CALL(E)                                          \
-  (R == 1   ? fk::ls::launch<E, 1>(a, share, sms, pdl, s)   \
-   : R == 2 ? fk::ls::launch<E, 2>(a, share, sms, pdl, s)   \
-   : R == 4 ? fk::ls::launch<E, 4>(a, share, sms, pdl, s)   \
-            : fk::ls::launch<E, 8>(a, share, sms, pdl, s))
-    if (share) return FK_BY_ELEM(e, FK_CALL);
+#define FK_CALL(E)                                              \
+  (R == 1   ? fk::ls::launch<E, 1>(a, plan, sms, err, pdl, s)   \
+   : R == 2 ? fk::ls::launch<E, 2>(a, plan, sms, err, pdl, s)   \
+   : R == 4 ? fk::ls::launch<E, 4>(a, plan, sms, err, pdl, s)   \
+            : fk::ls::launch<E, 8>(a, plan, sms, err, pdl, s))
+    if (plan.share) return FK_BY_ELEM(e, FK_CALL);
 #undef FK_CALL
   }
   return fk_launch_linear_mxfp4_tile(a, e, sms, err, pdl, s);
