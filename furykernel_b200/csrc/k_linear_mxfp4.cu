@@ -32,7 +32,6 @@ constexpr uint32_t kWarps = 16;
 constexpr uint32_t kThreads = 32 * kWarps;
 constexpr uint32_t kTileRows = 16;     // weight rows of a unit
 constexpr uint32_t kStageBlocks = 8;   // blocks of 32 weights a row a stage: 128 bytes of codes
-constexpr uint32_t kMaxStages = 4;     // a warp's own ring
 constexpr uint32_t kCodeBytes = kTileRows * kStageBlocks * 16;
 constexpr uint32_t kScaleWords = 3;    // the words that hold 8 bytes, wherever they start
 constexpr uint32_t kMaxPairs = 512;
@@ -40,6 +39,9 @@ constexpr uint32_t kMaxEntries = 4096;
 constexpr uint32_t kSmemBudget = 227 * 1024 - 1024;  // static and dynamic, less the alignment's slack
 
 enum { LS_TIMEOUT = 29 };  // a stage of codes never landed
+
+// Stages of a warp's own ring.
+__host__ __device__ constexpr uint32_t stages_of(uint32_t R) { return R <= 4 ? 3 : 2; }
 
 // A stage's scale words and their values as factors.
 constexpr uint32_t kScaleBytes = kTileRows * kScaleWords * 4;
@@ -50,13 +52,13 @@ constexpr uint32_t kFactorBytes = kTileRows * kStageBlocks * 4;
 __host__ __device__ constexpr uint32_t input_bytes(uint32_t steps, uint32_t R) {
   return steps * R * kStageBlocks * 128 + (steps * R * 4 + 15) / 16 * 16;
 }
-__host__ __device__ constexpr uint32_t warp_bytes(uint32_t steps, uint32_t R, uint32_t stages) {
-  return stages * (kCodeBytes + kScaleBytes) + kFactorBytes + input_bytes(steps, R);
+__host__ __device__ constexpr uint32_t warp_bytes(uint32_t steps, uint32_t R) {
+  return stages_of(R) * (kCodeBytes + kScaleBytes) + kFactorBytes + input_bytes(steps, R);
 }
 // Units whose sums wait together.
 __host__ __device__ constexpr uint32_t batch_of(uint32_t R) { return R <= 4 ? 8 : 4; }
 __host__ __device__ constexpr uint32_t static_bytes(uint32_t R) {
-  return kMaxPairs * 12 + kThreads * 4 + batch_of(R) * kWarps * kTileRows * R * 4 + 1024 + kWarps * kMaxStages * 8;
+  return kMaxPairs * 12 + kThreads * 4 + batch_of(R) * kWarps * kTileRows * R * 4 + 1024 + kWarps * stages_of(R) * 8;
 }
 
 // Four bytes, of which `have` are there (the others become 0).
@@ -90,12 +92,12 @@ struct Pass {
 // others.
 template <class E, int R>
 __global__ void __launch_bounds__(kThreads, 1)
-    stream_kernel(const __grid_constant__ CUtensorMap tw, const FkLinearMx a, uint32_t share, uint32_t stages,
+    stream_kernel(const __grid_constant__ CUtensorMap tw, const FkLinearMx a, uint32_t share,
                   long long wait_cycles, int* __restrict__ err) {
   constexpr int NT = (R + 3) / 4;  // products of 8 columns
-  constexpr uint32_t kBatch = batch_of(R);
+  constexpr uint32_t kBatch = batch_of(R), stages = stages_of(R);
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t landed[kWarps][kMaxStages];
+  __shared__ __align__(8) uint64_t landed[kWarps][stages];
   __shared__ Pass passes[kMaxPairs];
   __shared__ uint32_t perm[kMaxPairs];  // a pair's row, its rank << 16
   __shared__ uint32_t ids_s[kThreads];
@@ -110,7 +112,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t pairs = a.m * a.k, tiles = (a.n + kTileRows - 1) / kTileRows;
 
   // The weights too may be the previous launch's (quant_mxfp4's): nothing is read before it is done.
-  if (tid < kWarps * kMaxStages) mbar_init(smem_u32(&landed[0][0] + tid), 1);
+  if (tid < kWarps * stages) mbar_init(smem_u32(&landed[0][0] + tid), 1);
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   grid_wait();
   grid_launch_dependents();
@@ -190,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t s0 = part * all_steps / share, steps = (part + 1) * all_steps / share - s0;
   const uint64_t scale_bytes = (uint64_t)a.entries * a.n * blocks;
   const uint32_t ring = smem_u32(smem) + warp * stages * kCodeBytes;
-  uint8_t* mine_smem = rest_smem + warp * (warp_bytes(most_steps, R, stages) - stages * kCodeBytes);
+  uint8_t* mine_smem = rest_smem + warp * (warp_bytes(most_steps, R) - stages * kCodeBytes);
   const uint32_t scale_ring = smem_u32(mine_smem);
   float* factors = reinterpret_cast<float*>(mine_smem + stages * kScaleBytes);  // [16 rows][8]
   // The inputs, [blocks][R][4][2] 16 bytes as the products take them, and
@@ -198,50 +200,67 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* xs = reinterpret_cast<uint8_t*>(factors) + kFactorBytes;
   float* sxs = reinterpret_cast<float*>(xs + most_steps * kStageBlocks * R * 128);
 
-  // The loads of the next stage: the warp's own cursor over (unit, step).
-  // A unit's rows end with the table's: the last unit starts early enough
-  // (its first rows are another's too, with the same results).
+  // A unit's first row, and where this warp's scale bytes of row `of` of it
+  // start. A unit's rows end with the table's: the last unit starts early
+  // enough (its first rows are another's too, with the same results).
+  auto first_row = [&](uint32_t tile) { return min(tile * kTileRows, a.n - kTileRows); };
+  auto first_scale = [&](uint32_t pass, uint32_t tile, uint32_t of) {
+    return ((uint64_t)passes[pass].e * a.n + first_row(tile) + of) * blocks + s0 * kStageBlocks;
+  };
+
+  // The loads of the next stage: the warp's own cursor over (unit, step). A
+  // lane's scale word is word lane % 2 of the row's (the even lanes take
+  // word 2 too, where the bytes reach into it); the table's last word may
+  // be short. From one unit to the next of a pass all of it moves on by 16
+  // rows, whole words, but for the last.
   uint32_t left = steps ? u1 - u0 : 0, ltile = u0 % tiles, lpass = u0 / tiles, ls = 0, lslot = 0, issued = 0;
   const uint8_t* lsc = nullptr;
-  uint32_t lrest = 0, lrow = 0, lentry = 0;
-  int lword = 0;  // where the lane's word starts against its row's first byte
+  int lrest = 0, lx = 0, lrow = 0, lentry = 0;
+  bool third = false;
+  auto aim = [&]() {
+    const uint64_t first = first_scale(lpass, ltile, lane >> 1), word = (first & ~3ull) + 4 * (lane & 1);
+    lsc = a.scales + word;
+    lrest = word < scale_bytes ? (int)min(scale_bytes - word, (uint64_t)0x40000000u) : 0;
+    third = !(lane & 1) && (first & 3);
+    lrow = (int)first_row(ltile);
+    lentry = (int)passes[lpass].e;
+  };
+  const uint32_t scale_to = scale_ring + (lane >> 1) * kScaleWords * 4 + (lane & 1) * 4;
   auto load = [&]() {
     if (left) {
-      if (ls == 0) {
-        lentry = passes[lpass].e;
-        lrow = min(ltile * kTileRows, a.n - kTileRows);
-        const uint64_t first = ((uint64_t)lentry * a.n + lrow + (lane >> 1)) * blocks + s0 * kStageBlocks;
-        lword = (int)(4 * (lane & 1)) - (int)(first & 3);
-        const uint64_t word = (first & ~3ull) + 4 * (lane & 1);
-        lsc = a.scales + word;
-        lrest = (uint32_t)min(scale_bytes - min(word, scale_bytes), (uint64_t)0x40000000u);
-      }
       if (lane == 0) {
         const uint32_t bar = smem_u32(&landed[warp][lslot]);
         mbar_expect_tx(bar, kCodeBytes);
-        tma_load_3d(ring + lslot * kCodeBytes, &tw, (int)((s0 + ls) * kStageBlocks * 16), (int)lrow, (int)lentry, bar);
+        tma_load_3d(ring + lslot * kCodeBytes, &tw, lx, lrow, lentry, bar);
       }
-      // Words 0 and 1 of a row, and the third where its bytes reach into it
-      // (the even lanes); the table's last word may be short.
-      const int have = (int)min(blocks - (s0 + ls) * kStageBlocks, kStageBlocks);
-      const uint32_t to = scale_ring + lslot * kScaleBytes + (lane >> 1) * kScaleWords * 4;
-      if (lword < have) copy4(to + (lane & 1) * 4, lsc, min(4u, lrest));
-      if (!(lane & 1) && lword + 8 < have) copy4(to + 8, lsc + 8, min(4u, lrest - 8));
-      lsc += kStageBlocks, lrest -= kStageBlocks;
+      if (lrest > 0) copy4(scale_to + lslot * kScaleBytes, lsc, (uint32_t)min(4, lrest));
+      if (third && lrest > 8) copy4(scale_to + lslot * kScaleBytes + 8, lsc + 8, (uint32_t)min(4, lrest - 8));
+      lsc += kStageBlocks, lrest -= kStageBlocks, lx += kStageBlocks * 16;
       ++issued;
       if (++ls == steps) {
         ls = 0, --left;
+        lx = (int)(s0 * kStageBlocks * 16);
         if (++ltile == tiles) ltile = 0, ++lpass;
+        if (ltile != 0 && ltile + 1 != tiles) {
+          lsc += kTileRows * blocks - steps * kStageBlocks;
+          lrest -= (int)min(kTileRows * blocks - steps * kStageBlocks, (uint32_t)max(lrest, 0));
+          lrow += kTileRows;
+        } else if (left) {
+          aim();
+        }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     lslot = lslot + 1 == stages ? 0 : lslot + 1;
   };
+  lx = (int)(s0 * kStageBlocks * 16);
+  if (left) aim();
   __syncthreads();  // the barriers are ready
   for (uint32_t i = 0; i < stages - 1; ++i) load();
 
-  uint32_t slot = 0, phase = 0, held = 0, tile = u0 % tiles, pass = u0 / tiles;
+  uint32_t slot = 0, phase = 0, held = 0, shift = 0, tile = u0 % tiles, pass = u0 / tiles;
   bool lost = false;
+  const uint32_t ragged = blocks % kStageBlocks;
   auto group_sync = [&]() {
     if (share > 1)
       asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * share) : "memory");
@@ -281,10 +300,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
     }
-    const uint32_t r0 = min(tile * kTileRows, a.n - kTileRows);
     // Where the scale bytes of row lane / 2 lie in their words (a stage moves on by whole words).
-    const uint32_t shift =
-        8 * ((uint32_t)(((uint64_t)ps.e * a.n + r0 + (lane >> 1)) * blocks + s0 * kStageBlocks) & 3u);
+    if (tile == 0 || tile + 1 == tiles || u == u0) shift = 8 * ((uint32_t)first_scale(pass, tile, lane >> 1) & 3u);
     float acc[NT][2];
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = 0.0f;
@@ -294,16 +311,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float* sat = sxs + t % R;
     for (uint32_t step = 0; step < steps; ++step) {
       load();
-      // All groups but the last stages - 1 have landed.
-      if (stages == 4)
-        asm volatile("cp.async.wait_group 3;" ::: "memory");
-      else if (stages == 3)
-        asm volatile("cp.async.wait_group 2;" ::: "memory");
-      else
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-      if (!lost && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&landed[warp][slot]), phase, wait_cycles))) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(stages - 1) : "memory");  // all but the last ones
+      const uint32_t bar = smem_u32(&landed[warp][slot]);
+      if (!mbar_try(bar, phase) && !lost && !mbar_wait(bar, phase, wait_cycles)) {
         lost = true;  // the results are not to be used: the status says so
-        if (lane == 0) record(err, LS_TIMEOUT);
+        record(err, LS_TIMEOUT);
       }
       __syncwarp();
       // The stage's scales as factors, four blocks of one row a lane: a byte
@@ -312,7 +324,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t* w = reinterpret_cast<const uint32_t*>(mine_smem + slot * kScaleBytes) +
                             (lane >> 1) * kScaleWords + (lane & 1);
         uint32_t bytes = __funnelshift_r(w[0], w[1], shift);
-        const uint32_t have = blocks - (s0 + step) * kStageBlocks;
         float f[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -320,10 +331,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 __uint_as_float(0x00400000u));
           f[j] = fmaf(v, 0.0f, v);
         }
-        if (have < kStageBlocks) {  // the row ends in this stage: no factor past it
+        if (ragged && s0 + step + 1 == all_steps) {  // the row ends in this stage: no factor past it
 #pragma unroll
           for (uint32_t j = 0; j < 4; ++j)
-            if (4 * (lane & 1) + j >= have) f[j] = 0.0f;
+            if (4 * (lane & 1) + j >= ragged) f[j] = 0.0f;
         }
         reinterpret_cast<float4*>(factors)[lane] = make_float4(f[0], f[1], f[2], f[3]);
       }
@@ -388,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (uint32_t w = 1; w < share; ++w) v = __fadd_rn(v, from[w * (kTileRows * R)]);
       const uint32_t p = perm[po.first + (i >> 4)];
       mx::store<E>(static_cast<typename E::Storage*>(a.y) + (size_t)(p & 0xFFFFu) * a.ldy + (size_t)(p >> 16) * a.n +
-                       min(uo % tiles * kTileRows, a.n - kTileRows) + (i & 15),
+                       first_row(uo % tiles) + (i & 15),
                    v);
     }
     held = 0;
@@ -402,24 +413,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_wait(smem_u32(&landed[warp][i % stages]), (i / stages) & 1, wait_cycles);
 }
 
-// How many warps share a unit, and how many stages a warp's ring has.
-struct Plan {
-  uint32_t share, stages;
-};
-
-// The fewest rounds of units, each its blocks a warp and about 4 blocks'
-// worth of fixed cost, whose inputs fit beside two stages a warp or more.
-inline Plan plan_of(uint64_t units, uint32_t blocks, uint32_t R, int sms) {
-  Plan best = {0, 0};
+// How many warps share a unit: the fewest rounds of units, each its blocks
+// a warp and about 8 blocks' worth of fixed cost, whose inputs fit. 0: none.
+inline uint32_t share_of(uint64_t units, uint32_t blocks, uint32_t R, int sms) {
+  uint32_t best = 0;
   uint64_t least = ~0ull;
   const uint32_t all = (blocks + kStageBlocks - 1) / kStageBlocks;
   for (uint32_t share = kWarps; share >= 1; share /= 2) {
     const uint32_t steps = (all + share - 1) / share;
     const uint64_t at_once = (uint64_t)sms * (kWarps / share);
-    const uint64_t cost = (units + at_once - 1) / at_once * (steps * kStageBlocks + 4);
-    uint32_t stages = kMaxStages;
-    while (stages >= 2 && static_bytes(R) + (uint64_t)kWarps * warp_bytes(steps, R, stages) > kSmemBudget) --stages;
-    if (stages >= 2 && cost < least) least = cost, best = {share, stages};
+    const uint64_t cost = (units + at_once - 1) / at_once * (steps * kStageBlocks + 8);
+    if (static_bytes(R) + (uint64_t)kWarps * warp_bytes(steps, R) <= kSmemBudget && cost < least)
+      least = cost, best = share;
   }
   return best;
 }
@@ -445,19 +450,19 @@ inline bool code_map(CUtensorMap* map, const FkLinearMx& a) {
 }
 
 template <class E, int R>
-cudaError_t launch(const FkLinearMx& a, Plan plan, int sms, int* err, bool pdl, cudaStream_t s) {
+cudaError_t launch(const FkLinearMx& a, uint32_t share, int sms, int* err, bool pdl, cudaStream_t s) {
   const uint64_t pairs = (uint64_t)a.m * a.k, tiles = (a.n + kTileRows - 1) / kTileRows;
-  const uint32_t all = (a.kk / mx::kBlock + kStageBlocks - 1) / kStageBlocks, share = plan.share;
-  size_t rest = (size_t)kWarps * (warp_bytes((all + share - 1) / share, R, plan.stages) - plan.stages * kCodeBytes);
+  const uint32_t all = (a.kk / mx::kBlock + kStageBlocks - 1) / kStageBlocks;
+  size_t rest = (size_t)kWarps * (warp_bytes((all + share - 1) / share, R) - stages_of(R) * kCodeBytes);
   if (a.ids && rest < (a.entries + kThreads) * 4) rest = (a.entries + kThreads) * 4;  // the count's space
-  const size_t smem = 1024 + (size_t)kWarps * plan.stages * kCodeBytes + rest;
+  const size_t smem = 1024 + (size_t)kWarps * stages_of(R) * kCodeBytes + rest;
   CUtensorMap tw;
   if (!code_map(&tw, a)) return cudaErrorInvalidValue;
   cudaError_t e = fk_allow_smem(stream_kernel<E, R>, smem);
   if (e != cudaSuccess) return e;
   const uint64_t most = (pairs * tiles + kWarps / share - 1) / (kWarps / share);  // blocks that have a unit
   return fk_launch_ex(stream_kernel<E, R>, dim3((uint32_t)(most < (uint64_t)sms ? most : (uint64_t)sms)),
-                      dim3(kThreads), smem, s, pdl, tw, a, share, plan.stages, (long long)4000000000LL, err);
+                      dim3(kThreads), smem, s, pdl, tw, a, share, (long long)4000000000LL, err);
 }
 
 }  // namespace ls
@@ -478,19 +483,19 @@ cudaError_t fk_launch_linear_mxfp4(const FkLinearMx& a, FkElem e, int sms, int* 
     // Rows a pass: 4 where an expert has that many on average, 8 past it,
     // fewer where there are no more or where they do not fit.
     uint32_t R = pairs <= 2 ? (uint32_t)pairs : pairs <= 4ull * a.entries ? 4 : 8;
-    fk::ls::Plan plan = {0, 0};
+    uint32_t share = 0;
     const uint64_t experts = a.ids && pairs > a.entries ? a.entries : a.ids ? pairs : 1;  // at most
     for (; R >= 1; R /= 2) {
       const uint64_t passes = a.ids ? experts : (pairs + R - 1) / R;
-      plan = fk::ls::plan_of(passes * ((a.n + fk::ls::kTileRows - 1) / fk::ls::kTileRows), a.kk / 32, R, sms);
-      if (plan.share) break;
+      share = fk::ls::share_of(passes * ((a.n + fk::ls::kTileRows - 1) / fk::ls::kTileRows), a.kk / 32, R, sms);
+      if (share) break;
     }
 #define FK_CALL(E)                                              \
-  (R == 1   ? fk::ls::launch<E, 1>(a, plan, sms, err, pdl, s)   \
-   : R == 2 ? fk::ls::launch<E, 2>(a, plan, sms, err, pdl, s)   \
-   : R == 4 ? fk::ls::launch<E, 4>(a, plan, sms, err, pdl, s)   \
-            : fk::ls::launch<E, 8>(a, plan, sms, err, pdl, s))
-    if (plan.share) return FK_BY_ELEM(e, FK_CALL);
+  (R == 1   ? fk::ls::launch<E, 1>(a, share, sms, err, pdl, s)   \
+   : R == 2 ? fk::ls::launch<E, 2>(a, share, sms, err, pdl, s)   \
+   : R == 4 ? fk::ls::launch<E, 4>(a, share, sms, err, pdl, s)   \
+            : fk::ls::launch<E, 8>(a, share, sms, err, pdl, s))
+    if (share) return FK_BY_ELEM(e, FK_CALL);
 #undef FK_CALL
   }
   return fk_launch_linear_mxfp4_tile(a, e, sms, err, pdl, s);
