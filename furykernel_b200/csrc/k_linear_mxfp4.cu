@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint32_t ids_s[kThreads];
   __shared__ float red[kBatch][kWarps][kTileRows * R];
   __shared__ uint32_t sums[2][kWarps], npasses_s, nrest_s;
-  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (an offset, so that the loads stay shared memory's)
   const uint32_t blocks = a.kk / mx::kBlock, all_steps = (blocks + kStageBlocks - 1) / kStageBlocks;
   const uint32_t most_steps = (all_steps + share - 1) / share;
   // [kWarps][stages] codes, then a warp's scale words, factors and inputs.

@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr uint32_t kCols = 2 * N < 32 ? 32 : 2 * N;
   constexpr uint32_t kHalf = TN / 2;  // a drain warp's tokens
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (an offset, so that the loads stay shared memory's)
   uint8_t* xs = smem;                            // [S][N rows][128 bytes]
   uint8_t* ws = xs + S * N * 128;                // [S][128 rows][128 bytes]
   uint8_t* raw = ws + S * kRows * 128;           // [kRawStages][128 rows][128 bytes]
