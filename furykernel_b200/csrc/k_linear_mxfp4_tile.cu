@@ -42,10 +42,13 @@ constexpr uint32_t kRun = 512;    // K of a run
 constexpr uint32_t kRawK = 256;   // K of a stage of codes: 128 bytes
 constexpr uint32_t kThreads = 608;
 // Warps: 0..7 drain, 8..15 widen the weights, 16 loads inputs, 17 the MMAs, 18 loads codes.
-constexpr uint32_t kRawStages = 3;
-constexpr uint32_t kMaxStages = 4;
-constexpr uint32_t kScaleSlots = 8;
-constexpr uint32_t kSmemBudget = 222 * 1024;
+constexpr uint32_t kSets = 2;        // of four widening warps, which take slabs in turn
+constexpr uint32_t kRawStages = 2;
+constexpr uint32_t kWideStages = 3;  // of widened weights
+constexpr uint32_t kMaxStages = 6;   // of inputs
+constexpr uint32_t kDone = 8;        // slabs whose MMAs' end is told apart
+constexpr uint32_t kScaleSlots = 16;
+constexpr uint32_t kSmemBudget = 226 * 1024;
 constexpr uint32_t kMaxEntries = 4096;
 
 // Status codes (first one wins), after the TF32 GEMMs'.
@@ -137,11 +140,18 @@ __device__ __forceinline__ uint32_t top_byte(uint32_t w) {
   return max(w & 0xFFu, (w >> 8) & 0xFFu);
 }
 
-__host__ __device__ constexpr uint32_t stage_bytes(int parts, int tn) { return (uint32_t)(parts * tn) * 128 + kRows * 128; }
+// All but the inputs' stages: widened weights, codes, factors, each drain
+// warp's factors and output places, barriers, and the alignment's slack.
+__host__ __device__ constexpr uint32_t fixed_bytes(int tn) {
+  return (kWideStages + kRawStages) * kRows * 128 + kScaleSlots * kRows * 4 + 8 * (tn / 2) * 12 + 512 + 1024;
+}
 __host__ __device__ constexpr uint32_t stages_of(int parts, int tn) {
-  return (kSmemBudget - kRawStages * kRows * 128 - 16384) / stage_bytes(parts, tn) < kMaxStages
-             ? (kSmemBudget - kRawStages * kRows * 128 - 16384) / stage_bytes(parts, tn)
+  return (kSmemBudget - fixed_bytes(tn)) / (uint32_t)(parts * tn * 128) < kMaxStages
+             ? (kSmemBudget - fixed_bytes(tn)) / (uint32_t)(parts * tn * 128)
              : kMaxStages;
+}
+__host__ __device__ constexpr uint32_t smem_of(int parts, int tn) {
+  return fixed_bytes(tn) + stages_of(parts, tn) * (uint32_t)(parts * tn * 128);
 }
 
 template <class E, int PARTS, int TN>
@@ -155,13 +165,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (an offset, so that the loads stay shared memory's)
   uint8_t* xs = smem;                            // [S][N rows][128 bytes]
-  uint8_t* ws = xs + S * N * 128;                // [S][128 rows][128 bytes]
-  uint8_t* raw = ws + S * kRows * 128;           // [kRawStages][128 rows][128 bytes]
-  float* swb = reinterpret_cast<float*>(raw + kRawStages * kRows * 128);  // [kScaleSlots][128]
-  float* sxb = swb + kScaleSlots * kRows;                                // [8 drain warps][kHalf]
-  uint32_t* pair = reinterpret_cast<uint32_t*>(sxb + 8 * kHalf);          // [8 drain warps][kHalf]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(pair + 8 * kHalf);
-  uint64_t *xfull = bars, *wfull = xfull + S, *empty = wfull + S, *rfull = empty + S, *rempty = rfull + kRawStages,
+  uint8_t* ws = xs + S * N * 128;                // [kWideStages][128 rows][128 bytes]
+  uint8_t* raw = ws + kWideStages * kRows * 128; // [kRawStages][128 rows][128 bytes]
+  uint64_t* place = reinterpret_cast<uint64_t*>(raw + kRawStages * kRows * 128);  // [8 drain warps][kHalf]
+  float* swb = reinterpret_cast<float*>(place + 8 * kHalf);                      // [kScaleSlots][128]
+  float* sxb = swb + kScaleSlots * kRows;                                        // [8 drain warps][kHalf]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sxb + 8 * kHalf);
+  // full: a slab's inputs and widened weights; done: its MMAs; rfull and
+  // rempty: a stage of codes; afull and aempty: a run's sums; sfull: a run's
+  // factors.
+  uint64_t *full = bars, *done = full + kDone, *rfull = done + kDone, *rempty = rfull + kRawStages,
            *afull = rempty + kRawStages, *aempty = afull + 2, *sfull = aempty + 2, *fin = sfull + kScaleSlots;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fin + 1);
 
@@ -170,10 +183,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t raws = (a.kk + kRawK - 1) / kRawK;
 
   if (threadIdx.x == 0) {
-    for (uint32_t s = 0; s < S; ++s) {
-      mbar_init(smem_u32(&xfull[s]), 1);
-      mbar_init(smem_u32(&wfull[s]), 8);
-      mbar_init(smem_u32(&empty[s]), 1);
+    for (uint32_t s = 0; s < kDone; ++s) {
+      mbar_init(smem_u32(&full[s]), 5);  // the inputs' loads and a set's four warps
+      mbar_init(smem_u32(&done[s]), 1);
     }
     for (uint32_t s = 0; s < kRawStages; ++s) {
       mbar_init(smem_u32(&rfull[s]), 1);
@@ -204,10 +216,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   Tile o;
   // A wait by every lane of a warp, together; false once it ran out.
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
+    if (__all_sync(0xffffffffu, mbar_try(smem_u32(bar), parity))) return true;
     const bool ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, wait_cycles));
     if (!ok && lane == 0) record(err, code);
     return ok;
   };
+  // The same by one thread.
+  auto wait1 = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
+    if (mbar_try(smem_u32(bar), parity) || mbar_wait(smem_u32(bar), parity, wait_cycles)) return true;
+    record(err, code);
+    return false;
+  };
+  // Slab j's MMAs have finished.
+  auto done_bar = [&](uint32_t j) { return &done[j % kDone]; };
 
   if (warp < 8) {
     // Drain: warp w reads TMEM lanes 32 (w % 4).. (weight rows) of the
@@ -215,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // stores a token's 32 neighbouring outputs together.
     const uint32_t quarter = warp & 3, half = warp >> 2;
     float* mysx = sxb + warp * kHalf;
-    uint32_t* mypair = pair + warp * kHalf;
+    uint64_t* myplace = place + warp * kHalf;
     const uint32_t at = tmem + ((32 * quarter) << 16) + half * kHalf;
     uint32_t g = 0;  // runs so far
     bool ok = true;
@@ -226,7 +247,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       for (uint32_t c = lane; c < kHalf; c += 32) {
         const uint32_t slot = o.slot0 + half * kHalf + c;
-        mypair[c] = half * kHalf + c < o.count ? (a.perm ? __ldg(a.perm + slot) : slot) : 0xffffffffu;
+        if (half * kHalf + c < o.count) {
+          const uint32_t p = a.perm ? __ldg(a.perm + slot) : slot;
+          myplace[c] = (uint64_t)(p / a.k) * a.ldy + (uint64_t)(p % a.k) * a.n + o.row0 + 32 * quarter;
+        }
       }
       for (uint32_t run = 0; run < runs; ++run, ++g) {
         __syncwarp();
@@ -260,93 +284,100 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(smem_u32(&aempty[g & 1]));
       }
       if (!ok) break;
-      const uint32_t row = o.row0 + 32 * quarter + lane;
-      if (row < a.n) {
-        typename E::Storage* y = static_cast<typename E::Storage*>(a.y) + row;
+      if (o.row0 + 32 * quarter + lane < a.n) {
+        typename E::Storage* y = static_cast<typename E::Storage*>(a.y) + lane;
 #pragma unroll
-        for (uint32_t c = 0; c < kHalf; ++c) {
-          const uint32_t p = mypair[c];
-          if (p != 0xffffffffu) mx::store<E>(y + (size_t)(p / a.k) * a.ldy + (size_t)(p % a.k) * a.n, acc[c]);
-        }
+        for (uint32_t c = 0; c < kHalf; ++c)
+          if (half * kHalf + c < o.count) mx::store<E>(y + myplace[c], acc[c]);
       }
     }
   } else if (warp < 16) {
-    // Widen: thread (row, half) takes one block of 32 weights of each slab:
-    // 16 bytes of codes to 64 bytes of binary16, where the 128-byte swizzle
+    // Widen: two sets of four warps take slabs in turn, a thread a row: 32
+    // bytes of codes to 128 bytes of binary16, where the 128-byte swizzle
     // puts them (chunk c of row r at c ^ (r % 8)).
-    const uint32_t id = threadIdx.x - 256, row = id & 127, half = id >> 7;
+    const uint32_t id = threadIdx.x - 256, row = id & 127, set = id >> 7, turn = row & 7;
     const uint32_t nb = a.kk / mx::kBlock;
-    uint32_t i = 0, q = 0, g = 0;  // slabs, code stages, runs so far
+    const uint8_t* from = raw + row * 128;
+    uint8_t* to = ws + row * 128;
+    uint32_t i0 = 0, q = 0, g = 0;  // slabs of earlier tiles, code stages, runs so far
     bool ok = true;
-    for (uint32_t t = blockIdx.x; ok && tile_at<TN>(a, t, o); t += gridDim.x) {
+    for (uint32_t t = blockIdx.x; ok && tile_at<TN>(a, t, o); t += gridDim.x, i0 += slabs) {
       const uint8_t* srow = a.scales + ((size_t)o.e * a.n + min(o.row0 + row, a.n - 1)) * nb;
       uint4 next = load_scales(srow, 0, nb);
-      uint4 sc = next;
-      int ref = 0;
-      for (uint32_t slab = 0; slab < slabs; ++slab, ++i) {
-        const uint32_t in_run = slab % (kRun / kSlab);
-        if (in_run == 0) {
-          sc = next;
-          next = load_scales(srow, (slab + kRun / kSlab) * 2, nb);
-          ref = (int)max(max(top_byte(sc.x), top_byte(sc.y)), max(top_byte(sc.z), top_byte(sc.w)));
-          if (half == 0) {
-            // The factor back: 2^(ref - 127 - 12).
-            const int p = ref - 139;
-            swb[(g % kScaleSlots) * kRows + row] =
-                __uint_as_float(p >= -126 ? (uint32_t)(p + 127) << 23 : 1u << (p + 149));
+      for (uint32_t run = 0; ok && run < runs; ++run, ++g) {
+        const uint4 sc = next;
+        next = load_scales(srow, (run + 1) * (kRun / mx::kBlock), nb);
+        const int ref = (int)max(max(top_byte(sc.x), top_byte(sc.y)), max(top_byte(sc.z), top_byte(sc.w)));
+        if (set == 0) {
+          // The factor back: 2^(ref - 127 - 12).
+          const int p = ref - 139;
+          swb[(g % kScaleSlots) * kRows + row] =
+              __uint_as_float(p >= -126 ? (uint32_t)(p + 127) << 23 : 1u << (p + 149));
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sfull[g % kScaleSlots]));
+        }
+        // The set's half word of scales: blocks 2 slab, 2 slab + 1 of its slabs.
+        const uint32_t mine[4] = {sc.x >> (16 * set), sc.y >> (16 * set), sc.z >> (16 * set), sc.w >> (16 * set)};
+#pragma unroll
+        for (uint32_t j = 0; j < kRun / kSlab / kSets; ++j) {
+          const uint32_t slab = run * (kRun / kSlab) + kSets * j + set;
+          const uint32_t rs = q % kRawStages;
+          const bool staged = slab / 4 * 4 < slabs;  // there is a stage of codes here
+          if (j % 2 == 0 && staged && !(ok = wait(&rfull[rs], (q / kRawStages) & 1, LT_TIMEOUT_CODES))) break;
+          if (slab < slabs) {
+            const uint32_t i = i0 + slab, s = i % kWideStages;
+            const uint8_t* cf = from + rs * kRows * 128;
+            const uint32_t c = (kSets * j % 4 + set) * 2;  // the slab's first 16 bytes of the stage's 128
+            const uint4 c0 = *reinterpret_cast<const uint4*>(cf + ((c ^ turn) << 4));
+            const uint4 c1 = *reinterpret_cast<const uint4*>(cf + (((c + 1) ^ turn) << 4));
+            uint32_t by[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t byte = (mine[j] >> (8 * h)) & 0xFFu;
+              by[h] = byte == 255 ? 0x7E007E00u : half_power2((int)byte - ref + 12);
+            }
+            if (i >= kWideStages &&
+                !(ok = wait(done_bar(i - kWideStages), (i - kWideStages) / kDone & 1, LT_TIMEOUT_MMA)))
+              break;
+            uint8_t* wt = to + s * kRows * 128;
+            const uint32_t words[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+#pragma unroll
+            for (int w = 0; w < 8; ++w) {
+              uint32_t h[4];
+              mx::widen8_f16(words[w], h);
+#pragma unroll
+              for (int v = 0; v < 4; ++v) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[v]) : "r"(by[w / 4]));
+              *reinterpret_cast<uint4*>(wt + ((w ^ turn) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+            }
+            fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&sfull[g % kScaleSlots]));
+            if (lane == 0) mbar_arrive(smem_u32(&full[i % kDone]));
           }
-          ++g;
+          // After a stage of codes: every warp is done with it, those of a set that had none of it too.
+          if (j % 2 == 1 && staged) {
+            if (lane == 0) mbar_arrive(smem_u32(&rempty[rs]));
+            ++q;
+          }
         }
-        const uint32_t rs = q % kRawStages;
-        if (slab % 4 == 0 && !(ok = wait(&rfull[rs], (q / kRawStages) & 1, LT_TIMEOUT_CODES))) break;
-        const uint4 cw = *reinterpret_cast<const uint4*>(raw + rs * kRows * 128 + row * 128 +
-                                                         (((slab % 4) * 2 + half) ^ (row & 7)) * 16);
-        const uint32_t word = in_run < 4 ? (in_run < 2 ? sc.x : sc.y) : (in_run < 6 ? sc.z : sc.w);
-        const uint32_t byte = (word >> (8 * (2 * (in_run & 1) + half))) & 0xFFu;
-        const uint32_t by = byte == 255 ? 0x7E007E00u : half_power2((int)byte - ref + 12);
-        const uint32_t s = i % S;
-        if (i >= S && !(ok = wait(&empty[s], (i / S - 1) & 1, LT_TIMEOUT_MMA))) break;
-        uint8_t* to = ws + s * kRows * 128 + row * 128;
-        const uint32_t words[4] = {cw.x, cw.y, cw.z, cw.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t h[4];
-          mx::widen8_f16(words[j], h);
-#pragma unroll
-          for (int v = 0; v < 4; ++v) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[v]) : "r"(by));
-          *reinterpret_cast<uint4*>(to + ((4 * half + j) ^ (row & 7)) * 16) = make_uint4(h[0], h[1], h[2], h[3]);
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(smem_u32(&wfull[s]));
-          if (slab % 4 == 3 || slab + 1 == slabs) mbar_arrive(smem_u32(&rempty[rs]));
-        }
-        if (slab % 4 == 3 || slab + 1 == slabs) ++q;
       }
     }
   } else if (warp == 16 && lane == 0) {
     // Inputs: a slab's N rows, the parts one below the other.
-    uint32_t i = 0;
+    uint32_t i = 0, s = 0;
     bool ok = true;
     for (uint32_t t = blockIdx.x; ok && tile_at<TN>(a, t, o); t += gridDim.x)
       for (uint32_t slab = 0; slab < slabs; ++slab, ++i) {
-        const uint32_t s = i % S;
-        if (i >= S && !(ok = mbar_wait(smem_u32(&empty[s]), (i / S - 1) & 1, wait_cycles))) {
-          record(err, LT_TIMEOUT_MMA);
-          break;
-        }
-        const uint32_t bar = smem_u32(&xfull[s]);
+        if (i >= S && !(ok = wait1(done_bar(i - S), (i - S) / kDone & 1, LT_TIMEOUT_MMA))) break;
+        const uint32_t bar = smem_u32(&full[i % kDone]);
         mbar_expect_tx(bar, N * 128);
 #pragma unroll
         for (int p = 0; p < PARTS; ++p)
           tma_load_3d(smem_u32(xs + s * N * 128 + p * TN * 128), &tx, (int)(slab * kSlab), (int)o.slot0, p, bar);
+        s = s + 1 == S ? 0 : s + 1;
       }
-    // Loads in flight land before the CTA leaves.
-    for (uint32_t j = i > S ? i - S : 0; j < i; ++j)
-      if (!mbar_wait(smem_u32(&xfull[j % S]), (j / S) & 1, wait_cycles)) record(err, LT_TIMEOUT_INPUTS);
+    // Loads in flight land before the CTA leaves: the last slabs are done
+    // (or, where a wait ran out, their bytes have come, within limits).
+    for (uint32_t j = i > S ? i - S : 0; j < i; ++j) wait1(&full[j % kDone], j / kDone & 1, LT_TIMEOUT_INPUTS);
   } else if (warp == 18 && lane == 0) {
     // Codes: 256 of K a stage.
     uint32_t q = 0;
@@ -354,54 +385,40 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (uint32_t t = blockIdx.x; ok && tile_at<TN>(a, t, o); t += gridDim.x)
       for (uint32_t r = 0; r < raws; ++r, ++q) {
         const uint32_t s = q % kRawStages;
-        if (q >= kRawStages && !(ok = mbar_wait(smem_u32(&rempty[s]), (q / kRawStages - 1) & 1, wait_cycles))) {
-          record(err, LT_TIMEOUT_WIDEN);
-          break;
-        }
+        if (q >= kRawStages && !(ok = wait1(&rempty[s], (q / kRawStages - 1) & 1, LT_TIMEOUT_WIDEN))) break;
         const uint32_t bar = smem_u32(&rfull[s]);
         mbar_expect_tx(bar, kRows * 128);
         tma_load_3d(smem_u32(raw + s * kRows * 128), &tw, (int)(r * 128), (int)o.row0, (int)o.e, bar);
       }
     for (uint32_t j = q > kRawStages ? q - kRawStages : 0; j < q; ++j)
-      if (!mbar_wait(smem_u32(&rfull[j % kRawStages]), (j / kRawStages) & 1, wait_cycles))
-        record(err, LT_TIMEOUT_CODES);
+      wait1(&rfull[j % kRawStages], (j / kRawStages) & 1, LT_TIMEOUT_CODES);
   } else if (warp == 17 && lane == 0) {
-    const uint32_t idesc = f16_idesc(N);
-    uint32_t i = 0, g = 0;
+    constexpr uint32_t idesc = f16_idesc(N);
+    const uint64_t wd0 = sw128_desc(smem_u32(ws)), xd0 = sw128_desc(smem_u32(xs));
+    uint32_t i = 0, g = 0, s = 0, sw = 0;
     bool ok = true;
     for (uint32_t t = blockIdx.x; ok && tile_at<TN>(a, t, o); t += gridDim.x)
-      for (uint32_t slab = 0; slab < slabs; ++slab, ++i) {
-        const uint32_t in_run = slab % (kRun / kSlab), s = i % S;
-        if (in_run == 0) {
-          if (g >= 2 && !(ok = mbar_wait(smem_u32(&aempty[g & 1]), ((g >> 1) - 1) & 1, wait_cycles))) {
-            record(err, LT_TIMEOUT_DRAIN);
-            break;
-          }
-          fence_after();
-        }
-        if (!(ok = mbar_wait(smem_u32(&xfull[s]), (i / S) & 1, wait_cycles))) {
-          record(err, LT_TIMEOUT_INPUTS);
-          break;
-        }
-        if (!(ok = mbar_wait(smem_u32(&wfull[s]), (i / S) & 1, wait_cycles))) {
-          record(err, LT_TIMEOUT_WIDEN);
-          break;
-        }
+      for (uint32_t run = 0; ok && run < runs; ++run, ++g) {
+        if (g >= 2 && !(ok = wait1(&aempty[g & 1], ((g >> 1) - 1) & 1, LT_TIMEOUT_DRAIN))) break;
         fence_after();
-        const uint32_t wa = smem_u32(ws + s * kRows * 128), xa = smem_u32(xs + s * N * 128);
+        const uint32_t to = tmem + (g & 1) * N, end = min(kRun / kSlab, slabs - run * (kRun / kSlab));
+        for (uint32_t slab = 0; slab < end; ++slab, ++i) {
+          if (!(ok = wait1(&full[i % kDone], i / kDone & 1, LT_TIMEOUT_INPUTS))) break;
+          fence_after();
+          // A K step of 16 is 32 bytes of each row: 2 in a descriptor's address.
+          const uint64_t wd = wd0 + sw * (kRows * 128 / 16), xd = xd0 + s * (N * 128 / 16);
 #pragma unroll
-        for (uint32_t j = 0; j < kSlab / 16; ++j)
-          mma_f16(tmem + (g & 1) * N, sw128_desc(wa + 32 * j), sw128_desc(xa + 32 * j), idesc,
-                  in_run > 0 || j > 0 ? 1u : 0u);
-        mma_commit(smem_u32(&empty[s]));
-        if (in_run == kRun / kSlab - 1 || slab + 1 == slabs) {
-          mma_commit(smem_u32(&afull[g & 1]));
-          ++g;
+          for (uint32_t j = 0; j < kSlab / 16; ++j)
+            mma_f16(to, wd + 2 * j, xd + 2 * j, idesc, slab > 0 || j > 0 ? 1u : 0u);
+          mma_commit(smem_u32(done_bar(i)));
+          s = s + 1 == S ? 0 : s + 1;
+          sw = sw + 1 == kWideStages ? 0 : sw + 1;
         }
+        if (ok) mma_commit(smem_u32(&afull[g & 1]));
       }
     // Every MMA issued has finished before the CTA frees its tensor memory.
     mma_commit(smem_u32(fin));
-    if (!mbar_wait(smem_u32(fin), 0, wait_cycles)) record(err, LT_TIMEOUT_MMA);
+    wait1(fin, 0, LT_TIMEOUT_MMA);
   }
   fence_before();
   __syncthreads();
@@ -579,9 +596,7 @@ template <class E, int PARTS, int TN>
 cudaError_t launch_tile(const FkLinearMx& a, const fk::lt::Args& g, const uint16_t* parts, uint64_t most, int sms,
                         int* err, bool pdl, cudaStream_t s) {
   using namespace fk::lt;
-  constexpr uint32_t S = stages_of(PARTS, TN);
-  const size_t smem = 1024 + S * stage_bytes(PARTS, TN) + kRawStages * kRows * 128 + kScaleSlots * kRows * 4 +
-                      8 * (TN / 2) * 8 + (3 * S + 2 * kRawStages + 4 + kScaleSlots + 1) * 8 + 16;
+  constexpr size_t smem = smem_of(PARTS, TN);
   CUtensorMap tx, tw;
   if (!make_map_lt(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, parts, a.kk, g.slots, PARTS, kSlab, TN) ||
       !make_map_lt(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.kk / 2, a.n, a.entries, 128, kRows))
