@@ -38,6 +38,16 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
+// One thread of a converged warp, the same one each time. Code under its
+// branch is known to run in one thread, so that operands stay in uniform
+// registers: an MMA issued so costs 40 cycles of the thread's time, under
+// lane == 0 67 to 88 (measured on a B200).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t pred;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}\n" : "=r"(pred));
+  return pred != 0;
+}
+
 // Waits for the barrier's phase of the given parity, at most `cycles` SM
 // clock cycles; false on timeout.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, long long cycles) {

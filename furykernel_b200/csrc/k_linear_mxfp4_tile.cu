@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1)
            *afull = rempty + kRawStages, *aempty = afull + 2, *sfull = aempty + 2, *fin = sfull + kScaleSlots;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fin + 1);
 
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t slabs = (a.kk + kSlab - 1) / kSlab, runs = (a.kk + kRun - 1) / kRun;
   const uint32_t raws = (a.kk + kRawK - 1) / kRawK;
 
@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-  } else if (warp == 16 && lane == 0) {
+  } else if (warp == 16 && elect_one()) {
     // Inputs: a slab's N rows, the parts one below the other.
     uint32_t i = 0, s = 0;
     bool ok = true;
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Loads in flight land before the CTA leaves: the last slabs are done
     // (or, where a wait ran out, their bytes have come, within limits).
     for (uint32_t j = i > S ? i - S : 0; j < i; ++j) wait1(&full[j % kDone], j / kDone & 1, LT_TIMEOUT_INPUTS);
-  } else if (warp == 18 && lane == 0) {
+  } else if (warp == 18 && elect_one()) {
     // Codes: 256 of K a stage.
     uint32_t q = 0;
     bool ok = true;
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     for (uint32_t j = q > kRawStages ? q - kRawStages : 0; j < q; ++j)
       wait1(&rfull[j % kRawStages], (j / kRawStages) & 1, LT_TIMEOUT_CODES);
-  } else if (warp == 17 && lane == 0) {
+  } else if (warp == 17 && elect_one()) {
     constexpr uint32_t idesc = f16_idesc(N);
     const uint64_t wd0 = sw128_desc(smem_u32(ws)), xd0 = sw128_desc(smem_u32(xs));
     uint32_t i = 0, g = 0, s = 0, sw = 0;
