@@ -39,16 +39,27 @@ using namespace tc;
 constexpr uint32_t kRows = 128;   // weight rows a tile: the MMA's M, TMEM lanes
 constexpr uint32_t kSlab = 64;    // K of a stage: 128 bytes of binary16
 constexpr uint32_t kRun = 512;    // K of a run
-constexpr uint32_t kRawK = 256;   // K of a stage of codes: 128 bytes
-constexpr uint32_t kThreads = 608;
-// Warps: 0..7 drain, 8..15 widen the weights, 16 loads inputs, 17 the MMAs, 18 loads codes.
-constexpr uint32_t kSets = 2;        // of four widening warps, which take slabs in turn
-constexpr uint32_t kRawStages = 2;
-constexpr uint32_t kWideStages = 3;  // of widened weights
-constexpr uint32_t kMaxStages = 6;   // of inputs
-constexpr uint32_t kDone = 8;        // slabs whose MMAs' end is told apart
-constexpr uint32_t kScaleSlots = 16;
+constexpr uint32_t kPairK = 128;  // K of a stage of codes: 64 bytes, two slabs
+constexpr uint32_t kSets = 2;                       // of four widening warps, which take slabs in turn
+constexpr uint32_t kWidenWarps = 4 * kSets;
+constexpr uint32_t kInputWarp = 8 + kWidenWarps, kMmaWarp = kInputWarp + 1, kCodeWarp = kInputWarp + 2;
+constexpr uint32_t kThreads = 32 * (12 + kWidenWarps);
+// Warps: 0..7 drain, then the widening ones, then one that loads inputs, one
+// for the MMAs, one that loads codes and one idle. The launch gives each of
+// the 640 threads 96 registers (61440 in all); the drain warps, with a
+// tile's sums, take 128 and the others 72 (256 x 128 + 384 x 72 = 60416).
+constexpr uint32_t kDrainRegs = 128, kOtherRegs = 72;
+__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kDrainRegs)); }
+__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs)); }
+constexpr uint32_t kMaxStages = 6;    // of inputs
+constexpr uint32_t kDone = 8;         // slabs whose MMAs' end is told apart
+constexpr uint32_t kScaleSlots = 12;  // runs whose factors are held
 constexpr uint32_t kSmemBudget = 226 * 1024;
+// Stages of widened weights and of codes (even: a stage stays one set's):
+// what the widest tiles' inputs leave, else enough for two pairs of slabs a
+// set.
+__host__ __device__ constexpr uint32_t wide_stages(int n) { return n >= 256 ? 4 : 6; }
+__host__ __device__ constexpr uint32_t code_stages(int n) { return n >= 256 ? 2 : 6; }
 constexpr uint32_t kMaxEntries = 4096;
 
 // Status codes (first one wins), after the TF32 GEMMs'.
@@ -70,44 +81,66 @@ struct Args {
   const uint32_t* off;   // [entries + 1] first slot of each expert, or null: [0, m]
   const uint32_t* tpre;  // [entries + 1] first token tile of each expert
   const float* sx;       // [runs][slots] the inputs' factors
-  uint32_t entries, n, kk, k, ldy, slots, wtiles;
+  float* part;           // [2 grid][TN][128] sums of parts of tiles, or null: tiles stay whole
+  uint32_t* landed;      // [grid] parts written, of the tile that starts in this CTA
+  uint32_t entries, n, kk, k, ldy, slots, wtiles, runs;
 };
 
-struct Tile {
-  uint32_t e, slot0, count, row0;
+// Runs r0 .. r1 - 1 of a tile.
+struct Piece {
+  uint32_t e, slot0, count, row0, r0, r1, tile;
 };
 
-// Tile t: experts in order, of an expert the weight tiles in order, of a
-// weight tile the token tiles: CTAs that run together share weights.
+// A CTA's work: the tiles' runs in order (or whole tiles), an equal share of
+// neighbouring ones each. Experts in order, of an expert the weight tiles in
+// order, of a weight tile the token tiles, so that a CTA reads its weights
+// from HBM once.
 template <int TN>
-__device__ __forceinline__ bool tile_at(const Args& a, uint32_t t, Tile& o) {
-  const uint32_t q = t / a.wtiles;
-  uint32_t first = 0, tiles, s0 = 0, s1 = a.slots;
-  o.e = 0;
-  if (a.off) {
-    if (q >= __ldg(a.tpre + a.entries)) return false;
-    uint32_t lo = 0, hi = a.entries;  // the last expert whose first tile is <= q
-    while (hi - lo > 1) {
-      const uint32_t mid = (lo + hi) >> 1;
-      if (__ldg(a.tpre + mid) <= q)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    o.e = lo;
-    first = __ldg(a.tpre + lo);
-    s0 = __ldg(a.off + lo), s1 = __ldg(a.off + lo + 1);
-    tiles = __ldg(a.tpre + lo + 1) - first;
-  } else {
-    tiles = (a.slots + TN - 1) / TN;
-    if (q >= tiles) return false;
+struct Work {
+  uint32_t u, u1, units, per, ctas;  // this CTA's units and all of them, units a tile, CTAs that have any
+
+  __device__ __forceinline__ explicit Work(const Args& a) {
+    const uint32_t token_tiles = a.off ? __ldg(a.tpre + a.entries) : (a.slots + TN - 1) / TN;
+    per = a.part ? a.runs : 1;
+    units = token_tiles * a.wtiles * per;
+    ctas = min(gridDim.x, units);
+    u = blockIdx.x < ctas ? (uint32_t)((uint64_t)blockIdx.x * units / ctas) : 0;
+    u1 = blockIdx.x < ctas ? (uint32_t)((uint64_t)(blockIdx.x + 1) * units / ctas) : 0;
   }
-  const uint32_t local = t - first * a.wtiles;
-  o.slot0 = s0 + (local % tiles) * TN;
-  o.count = min((uint32_t)TN, s1 - o.slot0);
-  o.row0 = (local / tiles) * kRows;
-  return true;
-}
+  // The CTA that has unit v.
+  __device__ __forceinline__ uint32_t owner(uint32_t v) const {
+    return (uint32_t)((((uint64_t)v + 1) * ctas + units - 1) / units - 1);
+  }
+  __device__ __forceinline__ bool next(const Args& a, Piece& o) {
+    if (u >= u1) return false;
+    o.tile = u / per;
+    o.r0 = a.part ? u - o.tile * per : 0;
+    o.r1 = a.part ? min(per, o.r0 + (u1 - u)) : a.runs;
+    u += a.part ? o.r1 - o.r0 : 1;
+    const uint32_t q = o.tile / a.wtiles;
+    uint32_t first = 0, tiles = (a.slots + TN - 1) / TN, s0 = 0, s1 = a.slots;
+    o.e = 0;
+    if (a.off) {
+      uint32_t lo = 0, hi = a.entries;  // the last expert whose first tile is <= q
+      while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (__ldg(a.tpre + mid) <= q)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      o.e = lo;
+      first = __ldg(a.tpre + lo);
+      s0 = __ldg(a.off + lo), s1 = __ldg(a.off + lo + 1);
+      tiles = __ldg(a.tpre + lo + 1) - first;
+    }
+    const uint32_t local = o.tile - first * a.wtiles;
+    o.slot0 = s0 + (local % tiles) * TN;
+    o.count = min((uint32_t)TN, s1 - o.slot0);
+    o.row0 = (local / tiles) * kRows;
+    return true;
+  }
+};
 
 // Binary16 2^j as a pair, 0 below the type's range.
 __device__ __forceinline__ uint32_t half_power2(int j) {
@@ -116,12 +149,13 @@ __device__ __forceinline__ uint32_t half_power2(int j) {
 }
 
 // A row's 16 scale bytes of a run, from block b0 on; past the row's nb: 0.
+// Rows start on multiples of nb bytes.
 __device__ __forceinline__ uint4 load_scales(const uint8_t* row, uint32_t b0, uint32_t nb) {
   uint4 v = make_uint4(0, 0, 0, 0);
   if (b0 >= nb) return v;
-  if (nb % 16 == 0 && ((uintptr_t)row & 15) == 0) return __ldg(reinterpret_cast<const uint4*>(row + b0));
+  if (nb % 16 == 0) return __ldg(reinterpret_cast<const uint4*>(row + b0));
   uint32_t w[4] = {0, 0, 0, 0};
-  if (nb % 4 == 0 && ((uintptr_t)row & 3) == 0) {
+  if (nb % 4 == 0) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (b0 + 4 * i < nb) w[i] = __ldg(reinterpret_cast<const uint32_t*>(row + b0) + i);
@@ -133,25 +167,41 @@ __device__ __forceinline__ uint4 load_scales(const uint8_t* row, uint32_t b0, ui
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// The largest byte of a word, NaN scales (255) left out.
-__device__ __forceinline__ uint32_t top_byte(uint32_t w) {
-  w &= ~__vcmpeq4(w, 0xFFFFFFFFu);
-  w = __vmaxu4(w, w >> 16);
-  return max(w & 0xFFu, (w >> 8) & 0xFFu);
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// The largest of a run's 16 scale bytes, NaN's (255) left out.
+__device__ __forceinline__ uint32_t top_scale(const uint4& s) {
+  const uint32_t w[4] = {s.x, s.y, s.z, s.w};
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = max_u16x2(m, max_u16x2(w[i] & 0x00FF00FFu, (w[i] >> 8) & 0x00FF00FFu));
+  m = max(m & 0xFFFFu, m >> 16);
+  if (m == 255) {  // rare
+    m = 0;
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t b = (w[i / 4] >> (8 * (i % 4))) & 0xFFu;
+      if (b != 255) m = max(m, b);
+    }
+  }
+  return m;
 }
 
 // All but the inputs' stages: widened weights, codes, factors, each drain
-// warp's factors and output places, barriers, and the alignment's slack.
-__host__ __device__ constexpr uint32_t fixed_bytes(int tn) {
-  return (kWideStages + kRawStages) * kRows * 128 + kScaleSlots * kRows * 4 + 8 * (tn / 2) * 12 + 512 + 1024;
+// warp's factors, barriers, and the alignment's slack.
+__host__ __device__ constexpr uint32_t fixed_bytes(int parts, int tn) {
+  return wide_stages(parts * tn) * kRows * 128 + code_stages(parts * tn) * kRows * 64 + kScaleSlots * kRows * 4 +
+         8 * (tn / 2) * 4 + 512 + 1024;
 }
 __host__ __device__ constexpr uint32_t stages_of(int parts, int tn) {
-  return (kSmemBudget - fixed_bytes(tn)) / (uint32_t)(parts * tn * 128) < kMaxStages
-             ? (kSmemBudget - fixed_bytes(tn)) / (uint32_t)(parts * tn * 128)
+  return (kSmemBudget - fixed_bytes(parts, tn)) / (uint32_t)(parts * tn * 128) < kMaxStages
+             ? (kSmemBudget - fixed_bytes(parts, tn)) / (uint32_t)(parts * tn * 128)
              : kMaxStages;
 }
 __host__ __device__ constexpr uint32_t smem_of(int parts, int tn) {
-  return fixed_bytes(tn) + stages_of(parts, tn) * (uint32_t)(parts * tn * 128);
+  return fixed_bytes(parts, tn) + stages_of(parts, tn) * (uint32_t)(parts * tn * 128);
 }
 
 template <class E, int PARTS, int TN>
@@ -159,37 +209,36 @@ __global__ void __launch_bounds__(kThreads, 1)
     tile_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw, const Args a,
                 long long wait_cycles, int* __restrict__ err) {
   constexpr uint32_t N = PARTS * TN;  // the MMA's columns
-  constexpr uint32_t S = stages_of(PARTS, TN);
+  constexpr uint32_t S = stages_of(PARTS, TN), kWide = wide_stages(N), kCodes = code_stages(N);
   constexpr uint32_t kCols = 2 * N < 32 ? 32 : 2 * N;
   constexpr uint32_t kHalf = TN / 2;  // a drain warp's tokens
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (an offset, so that the loads stay shared memory's)
   uint8_t* xs = smem;                            // [S][N rows][128 bytes]
-  uint8_t* ws = xs + S * N * 128;                // [kWideStages][128 rows][128 bytes]
-  uint8_t* raw = ws + kWideStages * kRows * 128; // [kRawStages][128 rows][128 bytes]
-  uint64_t* place = reinterpret_cast<uint64_t*>(raw + kRawStages * kRows * 128);  // [8 drain warps][kHalf]
-  float* swb = reinterpret_cast<float*>(place + 8 * kHalf);                      // [kScaleSlots][128]
-  float* sxb = swb + kScaleSlots * kRows;                                        // [8 drain warps][kHalf]
+  uint8_t* ws = xs + S * N * 128;                // [kWide][128 rows][128 bytes]
+  uint8_t* raw = ws + kWide * kRows * 128;       // [kCodes][128 rows][64 bytes]
+  float* swb = reinterpret_cast<float*>(raw + kCodes * kRows * 64);  // [kScaleSlots][128]
+  float* sxb = swb + kScaleSlots * kRows;                            // [8 drain warps][kHalf]
   uint64_t* bars = reinterpret_cast<uint64_t*>(sxb + 8 * kHalf);
   // full: a slab's inputs and widened weights; done: its MMAs; rfull and
   // rempty: a stage of codes; afull and aempty: a run's sums; sfull: a run's
   // factors.
-  uint64_t *full = bars, *done = full + kDone, *rfull = done + kDone, *rempty = rfull + kRawStages,
-           *afull = rempty + kRawStages, *aempty = afull + 2, *sfull = aempty + 2, *fin = sfull + kScaleSlots;
+  uint64_t *full = bars, *done = full + kDone, *rfull = done + kDone, *rempty = rfull + kCodes,
+           *afull = rempty + kCodes, *aempty = afull + 2, *sfull = aempty + 2, *fin = sfull + kScaleSlots;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fin + 1);
 
   const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t slabs = (a.kk + kSlab - 1) / kSlab, runs = (a.kk + kRun - 1) / kRun;
-  const uint32_t raws = (a.kk + kRawK - 1) / kRawK;
+  const uint32_t slabs = (a.kk + kSlab - 1) / kSlab;
+  const uint32_t pairs = (a.kk + kPairK - 1) / kPairK;  // of slabs, the last perhaps one
 
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < kDone; ++s) {
       mbar_init(smem_u32(&full[s]), 5);  // the inputs' loads and a set's four warps
       mbar_init(smem_u32(&done[s]), 1);
     }
-    for (uint32_t s = 0; s < kRawStages; ++s) {
+    for (uint32_t s = 0; s < kCodes; ++s) {
       mbar_init(smem_u32(&rfull[s]), 1);
-      mbar_init(smem_u32(&rempty[s]), 8);
+      mbar_init(smem_u32(&rempty[s]), 4);
     }
     for (uint32_t s = 0; s < 2; ++s) {
       mbar_init(smem_u32(&afull[s]), 1);
@@ -200,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 17) {
+  if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(kCols)
                  : "memory");
@@ -213,7 +262,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   grid_wait();
   grid_launch_dependents();
 
-  Tile o;
+  __shared__ uint32_t arrived;
+  Work<TN> work(a);
+  Piece o;
   // A wait by every lane of a warp, together; false once it ran out.
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
     if (__all_sync(0xffffffffu, mbar_try(smem_u32(bar), parity))) return true;
@@ -231,37 +282,38 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto done_bar = [&](uint32_t j) { return &done[j % kDone]; };
 
   if (warp < 8) {
+    take_registers();
     // Drain: warp w reads TMEM lanes 32 (w % 4).. (weight rows) of the
     // tokens of its half, adds each run's sums, times both factors, and
     // stores a token's 32 neighbouring outputs together.
     const uint32_t quarter = warp & 3, half = warp >> 2;
     float* mysx = sxb + warp * kHalf;
-    uint64_t* myplace = place + warp * kHalf;
     const uint32_t at = tmem + ((32 * quarter) << 16) + half * kHalf;
     uint32_t g = 0;  // runs so far
-    bool ok = true;
-    for (uint32_t t = blockIdx.x; ok && tile_at<TN>(a, t, o); t += gridDim.x) {
+    bool ok = true;  // false: a wait ran out, the sums are not to be used (the status says so)
+    while (work.next(a, o)) {
       float acc[kHalf];
 #pragma unroll
       for (uint32_t c = 0; c < kHalf; ++c) acc[c] = 0.0f;
       __syncwarp();
-      for (uint32_t c = lane; c < kHalf; c += 32) {
-        const uint32_t slot = o.slot0 + half * kHalf + c;
-        if (half * kHalf + c < o.count) {
-          const uint32_t p = a.perm ? __ldg(a.perm + slot) : slot;
-          myplace[c] = (uint64_t)(p / a.k) * a.ldy + (uint64_t)(p % a.k) * a.n + o.row0 + 32 * quarter;
-        }
+      uint64_t place[(kHalf + 31) / 32];  // lane l: where tokens l, l + 32 of the half go
+#pragma unroll
+      for (uint32_t c = 0; c < kHalf; c += 32) {
+        const uint32_t in_tile = half * kHalf + c + lane, slot = o.slot0 + in_tile;
+        const bool live = c + lane < kHalf && in_tile < o.count;
+        const uint32_t p = live ? (a.perm ? __ldg(a.perm + slot) : slot) : 0;
+        place[c / 32] = (uint64_t)(p / a.k) * a.ldy + (uint64_t)(p % a.k) * a.n + o.row0 + 32 * quarter;
       }
-      for (uint32_t run = 0; run < runs; ++run, ++g) {
+      for (uint32_t run = o.r0; run < o.r1; ++run, ++g) {
         __syncwarp();
         for (uint32_t c = lane; c < kHalf; c += 32)
           mysx[c] = half * kHalf + c < o.count
                         ? __ldg(a.sx + (size_t)run * a.slots + o.slot0 + half * kHalf + c)
                         : 0.0f;
         __syncwarp();
-        if (!(ok = wait(&sfull[g % kScaleSlots], (g / kScaleSlots) & 1, LT_TIMEOUT_WIDEN))) break;
+        ok = ok && wait(&sfull[g % kScaleSlots], (g / kScaleSlots) & 1, LT_TIMEOUT_WIDEN);
         const float sw = swb[(g % kScaleSlots) * kRows + 32 * quarter + lane];
-        if (!(ok = wait(&afull[g & 1], (g >> 1) & 1, LT_TIMEOUT_MMA))) break;
+        ok = ok && wait(&afull[g & 1], (g >> 1) & 1, LT_TIMEOUT_MMA);
         fence_after();
         const uint32_t from = at + (g & 1) * N;
         constexpr uint32_t kPiece = kHalf < 16 ? kHalf : 16;
@@ -283,90 +335,142 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&aempty[g & 1]));
       }
-      if (!ok) break;
-      if (o.row0 + 32 * quarter + lane < a.n) {
-        typename E::Storage* y = static_cast<typename E::Storage*>(a.y) + lane;
+      if (o.r1 - o.r0 < a.runs) {
+        // A part of a tile: its sums to the workspace, by CTA and by whether
+        // the tile starts here; the last of the tile's CTAs to do so adds
+        // them all, in the CTAs' order.
+        constexpr size_t stride = (size_t)TN * kRows;
+        constexpr uint32_t kAtOnce = kHalf < 16 ? kHalf : 16;
+        const uint32_t first = o.tile * a.runs;
+        const uint32_t c0 = work.owner(first), c1 = work.owner(first + a.runs - 1);
+        const size_t mine = (size_t)(half * kHalf) * kRows + 32 * quarter + lane;
+        float* to = a.part + (2 * (size_t)blockIdx.x + (o.r0 == 0 ? 1 : 0)) * stride + mine;
 #pragma unroll
-        for (uint32_t c = 0; c < kHalf; ++c)
-          if (half * kHalf + c < o.count) mx::store<E>(y + myplace[c], acc[c]);
+        for (uint32_t c = 0; c < kHalf; ++c) to[c * kRows] = acc[c];
+        __threadfence();
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (threadIdx.x == 0) arrived = atomicAdd(a.landed + c0, 1u);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (arrived != c1 - c0) continue;
+        __threadfence();
+#pragma unroll
+        for (uint32_t c = 0; c < kHalf; ++c) acc[c] = __ldcg(a.part + (2 * (size_t)c0 + 1) * stride + mine + c * kRows);
+        for (uint32_t j = c0 + 1; j <= c1; ++j) {
+          const float* more = a.part + 2 * (size_t)j * stride + mine;
+#pragma unroll
+          for (uint32_t c = 0; c < kHalf; c += kAtOnce) {
+            float v[kAtOnce];
+#pragma unroll
+            for (uint32_t d = 0; d < kAtOnce; ++d) v[d] = __ldcg(more + (c + d) * kRows);
+#pragma unroll
+            for (uint32_t d = 0; d < kAtOnce; ++d) acc[c + d] = __fadd_rn(acc[c + d], v[d]);
+          }
+        }
+      }
+      typename E::Storage* y = static_cast<typename E::Storage*>(a.y) + lane;
+      const bool live = o.row0 + 32 * quarter + lane < a.n;
+#pragma unroll
+      for (uint32_t c = 0; c < kHalf; ++c) {
+        const uint64_t to = __shfl_sync(0xffffffffu, place[c / 32], c % 32);
+        if (live && half * kHalf + c < o.count) mx::store<E>(y + to, acc[c]);
       }
     }
-  } else if (warp < 16) {
-    // Widen: two sets of four warps take slabs in turn, a thread a row: 32
-    // bytes of codes to 128 bytes of binary16, where the 128-byte swizzle
-    // puts them (chunk c of row r at c ^ (r % 8)).
+  } else if (warp < 8 + kWidenWarps) {
+    give_registers();
+    // Widen: sets of four warps take pairs of slabs in turn, a thread a row:
+    // 64 bytes of codes to twice 128 bytes of binary16, where the 128-byte
+    // swizzle puts them (chunk c of row r at c ^ (r % 8); a codes' chunk at
+    // c ^ (r / 2 % 4)).
     const uint32_t id = threadIdx.x - 256, row = id & 127, set = id >> 7, turn = row & 7;
     const uint32_t nb = a.kk / mx::kBlock;
-    const uint8_t* from = raw + row * 128;
+    const uint8_t* from = raw + row * 64;
     uint8_t* to = ws + row * 128;
-    uint32_t i0 = 0, q = 0, g = 0;  // slabs of earlier tiles, code stages, runs so far
-    bool ok = true;
-    for (uint32_t t = blockIdx.x; ok && tile_at<TN>(a, t, o); t += gridDim.x, i0 += slabs) {
-      const uint8_t* srow = a.scales + ((size_t)o.e * a.n + min(o.row0 + row, a.n - 1)) * nb;
-      uint4 next = load_scales(srow, 0, nb);
-      for (uint32_t run = 0; ok && run < runs; ++run, ++g) {
+    uint32_t i = 0, s = 0, q = 0, g = 0;  // slabs so far, their place in the ring, pairs, runs
+    auto scales_of = [&](const Piece& p) {
+      return a.scales + ((size_t)p.e * a.n + min(p.row0 + row, a.n - 1)) * nb;
+    };
+    bool ok = true, more = work.next(a, o);
+    const uint8_t* srow = nullptr;
+    uint4 next = make_uint4(0, 0, 0, 0);
+    if (more) {
+      srow = scales_of(o);
+      next = load_scales(srow, o.r0 * (kRun / mx::kBlock), nb);
+    }
+    while (ok && more) {
+      const Piece p = o;
+      const uint8_t* prow = srow;
+      more = work.next(a, o);
+      if (more) srow = scales_of(o);
+      for (uint32_t run = p.r0; ok && run < p.r1; ++run, ++g) {
+        // A run's scales are loaded one run ahead, the next piece's first too.
         const uint4 sc = next;
-        next = load_scales(srow, (run + 1) * (kRun / mx::kBlock), nb);
-        const int ref = (int)max(max(top_byte(sc.x), top_byte(sc.y)), max(top_byte(sc.z), top_byte(sc.w)));
+        if (run + 1 < p.r1)
+          next = load_scales(prow, (run + 1) * (kRun / mx::kBlock), nb);
+        else if (more)
+          next = load_scales(srow, o.r0 * (kRun / mx::kBlock), nb);
+        const int ref = (int)top_scale(sc);
         if (set == 0) {
           // The factor back: 2^(ref - 127 - 12).
-          const int p = ref - 139;
+          const int p2 = ref - 139;
           swb[(g % kScaleSlots) * kRows + row] =
-              __uint_as_float(p >= -126 ? (uint32_t)(p + 127) << 23 : 1u << (p + 149));
+              __uint_as_float(p2 >= -126 ? (uint32_t)(p2 + 127) << 23 : 1u << (p2 + 149));
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&sfull[g % kScaleSlots]));
         }
-        // The set's half word of scales: blocks 2 slab, 2 slab + 1 of its slabs.
-        const uint32_t mine[4] = {sc.x >> (16 * set), sc.y >> (16 * set), sc.z >> (16 * set), sc.w >> (16 * set)};
+        const uint32_t end = min((run + 1) * (kRun / kPairK), pairs);
+#pragma unroll 1
+        for (uint32_t d = run * (kRun / kPairK); d < end; ++d, ++q) {
+          const bool two = 2 * d + 1 < slabs;
+          if (q % kSets == set) {
+            const uint32_t rs = q % kCodes, turn4 = (row >> 1) & 3, w = d % 4;
+            const uint32_t four = w < 2 ? (w == 0 ? sc.x : sc.y) : (w == 2 ? sc.z : sc.w);  // the blocks' scales
+            if (!(ok = wait(&rfull[rs], (q / kCodes) & 1, LT_TIMEOUT_CODES))) break;
+            uint4 codes[4];
 #pragma unroll
-        for (uint32_t j = 0; j < kRun / kSlab / kSets; ++j) {
-          const uint32_t slab = run * (kRun / kSlab) + kSets * j + set;
-          const uint32_t rs = q % kRawStages;
-          const bool staged = slab / 4 * 4 < slabs;  // there is a stage of codes here
-          if (j % 2 == 0 && staged && !(ok = wait(&rfull[rs], (q / kRawStages) & 1, LT_TIMEOUT_CODES))) break;
-          if (slab < slabs) {
-            const uint32_t i = i0 + slab, s = i % kWideStages;
-            const uint8_t* cf = from + rs * kRows * 128;
-            const uint32_t c = (kSets * j % 4 + set) * 2;  // the slab's first 16 bytes of the stage's 128
-            const uint4 c0 = *reinterpret_cast<const uint4*>(cf + ((c ^ turn) << 4));
-            const uint4 c1 = *reinterpret_cast<const uint4*>(cf + (((c + 1) ^ turn) << 4));
-            uint32_t by[2];
+            for (uint32_t c = 0; c < 4; ++c)
+              codes[c] = *reinterpret_cast<const uint4*>(from + rs * kRows * 64 + ((c ^ turn4) << 4));
+            // Both slabs' places are free once the slab before the second's last use is done.
+            const uint32_t before = i + 1 - kWide;
+            if (i + 1 >= kWide && !(ok = wait(done_bar(before), before / kDone & 1, LT_TIMEOUT_MMA))) break;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t byte = (mine[j] >> (8 * h)) & 0xFFu;
-              by[h] = byte == 255 ? 0x7E007E00u : half_power2((int)byte - ref + 12);
-            }
-            if (i >= kWideStages &&
-                !(ok = wait(done_bar(i - kWideStages), (i - kWideStages) / kDone & 1, LT_TIMEOUT_MMA)))
-              break;
-            uint8_t* wt = to + s * kRows * 128;
-            const uint32_t words[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+            for (uint32_t c = 0; c < 4; ++c) {
+              if (c == 2 && !two) break;
+              const uint32_t byte = (four >> (8 * c)) & 0xFFu;
+              const uint32_t by = byte == 255 ? 0x7E007E00u : half_power2((int)byte - ref + 12);
+              const uint32_t at = c < 2 ? s : s + 1 == kWide ? 0 : s + 1;
+              const uint32_t words[4] = {codes[c].x, codes[c].y, codes[c].z, codes[c].w};
 #pragma unroll
-            for (int w = 0; w < 8; ++w) {
-              uint32_t h[4];
-              mx::widen8_f16(words[w], h);
+              for (uint32_t v = 0; v < 4; ++v) {
+                uint32_t h[4];
+                mx::widen8_f16(words[v], h);
 #pragma unroll
-              for (int v = 0; v < 4; ++v) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[v]) : "r"(by[w / 4]));
-              *reinterpret_cast<uint4*>(wt + ((w ^ turn) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+                for (int u = 0; u < 4; ++u) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[u]) : "r"(by));
+                *reinterpret_cast<uint4*>(to + at * kRows * 128 + (((c % 2 * 4 + v) ^ turn) << 4)) =
+                    make_uint4(h[0], h[1], h[2], h[3]);
+              }
             }
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&full[i % kDone]));
+            if (lane == 0) {
+              mbar_arrive(smem_u32(&full[i % kDone]));
+              if (two) mbar_arrive(smem_u32(&full[(i + 1) % kDone]));
+              mbar_arrive(smem_u32(&rempty[rs]));
+            }
           }
-          // After a stage of codes: every warp is done with it, those of a set that had none of it too.
-          if (j % 2 == 1 && staged) {
-            if (lane == 0) mbar_arrive(smem_u32(&rempty[rs]));
-            ++q;
-          }
+          i += two ? 2 : 1;
+          s += two ? 2 : 1;
+          if (s >= kWide) s -= kWide;
         }
       }
     }
-  } else if (warp == 16 && elect_one()) {
+  } else {
+  give_registers();
+  if (warp == kInputWarp && elect_one()) {
     // Inputs: a slab's N rows, the parts one below the other.
     uint32_t i = 0, s = 0;
     bool ok = true;
-    for (uint32_t t = blockIdx.x; ok && tile_at<TN>(a, t, o); t += gridDim.x)
-      for (uint32_t slab = 0; slab < slabs; ++slab, ++i) {
+    while (ok && work.next(a, o))
+      for (uint32_t slab = o.r0 * (kRun / kSlab), end = min(o.r1 * (kRun / kSlab), slabs); slab < end; ++slab, ++i) {
         if (i >= S && !(ok = wait1(done_bar(i - S), (i - S) / kDone & 1, LT_TIMEOUT_MMA))) break;
         const uint32_t bar = smem_u32(&full[i % kDone]);
         mbar_expect_tx(bar, N * 128);
@@ -378,27 +482,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Loads in flight land before the CTA leaves: the last slabs are done
     // (or, where a wait ran out, their bytes have come, within limits).
     for (uint32_t j = i > S ? i - S : 0; j < i; ++j) wait1(&full[j % kDone], j / kDone & 1, LT_TIMEOUT_INPUTS);
-  } else if (warp == 18 && elect_one()) {
-    // Codes: 256 of K a stage.
+  } else if (warp == kCodeWarp && elect_one()) {
+    // Codes: a pair of slabs a stage.
     uint32_t q = 0;
     bool ok = true;
-    for (uint32_t t = blockIdx.x; ok && tile_at<TN>(a, t, o); t += gridDim.x)
-      for (uint32_t r = 0; r < raws; ++r, ++q) {
-        const uint32_t s = q % kRawStages;
-        if (q >= kRawStages && !(ok = wait1(&rempty[s], (q / kRawStages - 1) & 1, LT_TIMEOUT_WIDEN))) break;
+    while (ok && work.next(a, o))
+      for (uint32_t r = o.r0 * (kRun / kPairK), end = min(o.r1 * (kRun / kPairK), pairs); r < end; ++r, ++q) {
+        const uint32_t s = q % kCodes;
+        if (q >= kCodes && !(ok = wait1(&rempty[s], (q / kCodes - 1) & 1, LT_TIMEOUT_WIDEN))) break;
         const uint32_t bar = smem_u32(&rfull[s]);
-        mbar_expect_tx(bar, kRows * 128);
-        tma_load_3d(smem_u32(raw + s * kRows * 128), &tw, (int)(r * 128), (int)o.row0, (int)o.e, bar);
+        mbar_expect_tx(bar, kRows * 64);
+        tma_load_3d(smem_u32(raw + s * kRows * 64), &tw, (int)(r * 64), (int)o.row0, (int)o.e, bar);
       }
-    for (uint32_t j = q > kRawStages ? q - kRawStages : 0; j < q; ++j)
-      wait1(&rfull[j % kRawStages], (j / kRawStages) & 1, LT_TIMEOUT_CODES);
-  } else if (warp == 17 && elect_one()) {
+    for (uint32_t j = q > kCodes ? q - kCodes : 0; j < q; ++j)
+      wait1(&rfull[j % kCodes], (j / kCodes) & 1, LT_TIMEOUT_CODES);
+  } else if (warp == kMmaWarp && elect_one()) {
     constexpr uint32_t idesc = f16_idesc(N);
     const uint64_t wd0 = sw128_desc(smem_u32(ws)), xd0 = sw128_desc(smem_u32(xs));
     uint32_t i = 0, g = 0, s = 0, sw = 0;
     bool ok = true;
-    for (uint32_t t = blockIdx.x; ok && tile_at<TN>(a, t, o); t += gridDim.x)
-      for (uint32_t run = 0; ok && run < runs; ++run, ++g) {
+    while (ok && work.next(a, o))
+      for (uint32_t run = o.r0; ok && run < o.r1; ++run, ++g) {
         if (g >= 2 && !(ok = wait1(&aempty[g & 1], ((g >> 1) - 1) & 1, LT_TIMEOUT_DRAIN))) break;
         fence_after();
         const uint32_t to = tmem + (g & 1) * N, end = min(kRun / kSlab, slabs - run * (kRun / kSlab));
@@ -412,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mma_f16(to, wd + 2 * j, xd + 2 * j, idesc, slab > 0 || j > 0 ? 1u : 0u);
           mma_commit(smem_u32(done_bar(i)));
           s = s + 1 == S ? 0 : s + 1;
-          sw = sw + 1 == kWideStages ? 0 : sw + 1;
+          sw = sw + 1 == kWide ? 0 : sw + 1;
         }
         if (ok) mma_commit(smem_u32(&afull[g & 1]));
       }
@@ -420,10 +524,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     mma_commit(smem_u32(fin));
     wait1(fin, 0, LT_TIMEOUT_MMA);
   }
+  }
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == 17)
+  if (warp == kMmaWarp)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
 }
 
@@ -508,7 +613,8 @@ struct SplitArgs {
   float* sx;        // [runs][slots]
   const uint32_t* perm;
   const uint32_t* off;
-  uint32_t entries, n, kk, k, ldx, ldy, slots, runs;
+  uint32_t* landed;  // [grid] set to 0
+  uint32_t entries, n, kk, k, ldx, ldy, slots, runs, grid;
   bool per_rank;
 };
 
@@ -518,6 +624,8 @@ __global__ void __launch_bounds__(256) split_kernel(SplitArgs a) {
   grid_wait();
   grid_launch_dependents();
   const uint32_t lane = threadIdx.x & 31;
+  if (blockIdx.x == 0)
+    for (uint32_t c = threadIdx.x; c < a.grid; c += 256) a.landed[c] = 0;
   const uint64_t unit = blockIdx.x * 8ull + (threadIdx.x >> 5);
   if (unit >= (uint64_t)a.slots * a.runs) return;
   const uint32_t slot = (uint32_t)(unit / a.runs), run = (uint32_t)(unit % a.runs);
@@ -577,10 +685,10 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn_lt() {
   return fn;
 }
 
-// [depth][rows][width] elements as boxes of box_w x box_rows x 1, 128-byte
-// swizzle; what lies past any of the three reads as zeros.
+// [depth][rows][width] elements as boxes of box_w x box_rows x 1, swizzled
+// over 128 or 64 bytes; what lies past any of the three reads as zeros.
 bool make_map_lt(CUtensorMap* map, CUtensorMapDataType type, uint32_t elem, const void* base, uint64_t width,
-                 uint64_t rows, uint64_t depth, uint32_t box_w, uint32_t box_rows) {
+                 uint64_t rows, uint64_t depth, uint32_t box_w, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
   auto fn = encode_fn_lt();
   if (!fn) return false;
   cuuint64_t dims[3] = {width, rows, depth};
@@ -588,23 +696,24 @@ bool make_map_lt(CUtensorMap* map, CUtensorMapDataType type, uint32_t elem, cons
   cuuint32_t box[3] = {box_w, box_rows, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   return fn(map, type, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <class E, int PARTS, int TN>
-cudaError_t launch_tile(const FkLinearMx& a, const fk::lt::Args& g, const uint16_t* parts, uint64_t most, int sms,
-                        int* err, bool pdl, cudaStream_t s) {
+cudaError_t launch_tile(const FkLinearMx& a, const fk::lt::Args& g, const uint16_t* parts, uint32_t grid, int* err,
+                        bool pdl, cudaStream_t s) {
   using namespace fk::lt;
   constexpr size_t smem = smem_of(PARTS, TN);
   CUtensorMap tx, tw;
-  if (!make_map_lt(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, parts, a.kk, g.slots, PARTS, kSlab, TN) ||
-      !make_map_lt(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.kk / 2, a.n, a.entries, 128, kRows))
+  if (!make_map_lt(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, parts, a.kk, g.slots, PARTS, kSlab, TN,
+                   CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_map_lt(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.kk / 2, a.n, a.entries, kPairK / 2, kRows,
+                   CU_TENSOR_MAP_SWIZZLE_64B))
     return cudaErrorInvalidValue;
   cudaError_t e = fk_allow_smem(tile_kernel<E, PARTS, TN>, smem < 120 * 1024 ? 120 * 1024 : smem);
   if (e != cudaSuccess) return e;
-  const uint64_t grid = most < (uint64_t)sms ? most : (uint64_t)sms;
-  return fk_launch_ex(tile_kernel<E, PARTS, TN>, dim3((uint32_t)grid), dim3(kThreads),
+  return fk_launch_ex(tile_kernel<E, PARTS, TN>, dim3(grid), dim3(kThreads),
                       smem < 120 * 1024 ? (size_t)120 * 1024 : smem, s, pdl, tx, tw, g, (long long)4000000000LL, err);
 }
 
@@ -638,19 +747,34 @@ cudaError_t launch_all(const FkLinearMx& a, int sms, int* err, bool pdl, cudaStr
                                  off, tpre, perm);
     if (e != cudaSuccess) return e;
   }
-  SplitArgs sp = {a.x, a.y, parts, sx, perm, off, a.entries, a.n, a.kk, a.k, a.ldx, a.ldy, (uint32_t)pairs, runs,
-                  a.per_rank};
+  // A CTA an SM, each an equal share of the tiles' runs, where the parts of
+  // tiles that they leave find room in the workspace; else of whole tiles.
+  const uint32_t wtiles = (a.n + kRows - 1) / kRows;
+  const uint64_t most =
+      (a.ids ? pairs / tn + (pairs < a.entries ? pairs : (uint64_t)a.entries) : (pairs + tn - 1) / tn) * wtiles;  // tiles at most
+  uint64_t grid = most < (uint64_t)sms ? most : (uint64_t)sms;
+  uint32_t* landed = reinterpret_cast<uint32_t*>(take(4 * (uint64_t)sms));
+  const uint64_t left = fk_linear_mxfp4_work(a.entries, a.n, a.kk, a.m, a.k) -
+                        (uint64_t)(at - static_cast<uint8_t*>(a.work));
+  uint64_t split = most * runs < (uint64_t)sms ? most * runs : (uint64_t)sms;
+  if (split * 2 * tn * kRows * 4 > left) split = left / (2 * tn * kRows * 4);
+  float* part = nullptr;
+  if (split >= grid && runs > 1 && most * runs < 0x80000000ull) {
+    grid = split;
+    part = reinterpret_cast<float*>(at);
+  }
+  SplitArgs sp = {a.x,    a.y,   parts, sx,    perm,  off,   landed,          a.entries, a.n,
+                  a.kk,   a.k,   a.ldx, a.ldy, (uint32_t)pairs, runs, (uint32_t)grid,  a.per_rank};
   const uint64_t blocks = (pairs * runs + 7) / 8;
   cudaError_t e = fk_launch_ex(split_kernel<E, PARTS>, dim3((uint32_t)blocks), dim3(256), 0, s, pdl, sp);
   if (e != cudaSuccess) return e;
-  Args g = {a.scales, a.y, perm, off, tpre, sx, a.entries, a.n, a.kk, a.k, a.ldy, (uint32_t)pairs,
-            (a.n + kRows - 1) / kRows};
-  const uint64_t most =
-      (pairs / tn + (a.ids ? (pairs < a.entries ? pairs : (uint64_t)a.entries) : 1)) * g.wtiles;  // tiles at most
-  if (tn == 16) return launch_tile<E, PARTS, 16>(a, g, parts, most, sms, err, pdl, s);
-  if (tn == 32) return launch_tile<E, PARTS, 32>(a, g, parts, most, sms, err, pdl, s);
-  if (tn == 64) return launch_tile<E, PARTS, 64>(a, g, parts, most, sms, err, pdl, s);
-  return launch_tile<E, PARTS, 128>(a, g, parts, most, sms, err, pdl, s);
+  Args g = {a.scales, a.y, perm, off,   tpre,            sx,     part, landed, a.entries,
+            a.n,      a.kk, a.k, a.ldy, (uint32_t)pairs, wtiles, runs};
+  const uint32_t ctas = (uint32_t)grid;
+  if (tn == 16) return launch_tile<E, PARTS, 16>(a, g, parts, ctas, err, pdl, s);
+  if (tn == 32) return launch_tile<E, PARTS, 32>(a, g, parts, ctas, err, pdl, s);
+  if (tn == 64) return launch_tile<E, PARTS, 64>(a, g, parts, ctas, err, pdl, s);
+  return launch_tile<E, PARTS, 128>(a, g, parts, ctas, err, pdl, s);
 }
 
 }  // namespace
