@@ -9,6 +9,7 @@
 // the type's largest: 1 to 3 significant bits.
 #pragma once
 
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
 
@@ -120,8 +121,25 @@ template <class E>
 __device__ __forceinline__ void store(typename E::Storage* p, float v) {
   if constexpr (E::kElem == FK_F32)
     *p = v;
+  else if constexpr (E::kElem == FK_BF16)
+    *p = __bfloat16_as_ushort(__float2bfloat16_rn(v));
   else
-    *p = E::narrow(v);
+    *p = __half_as_ushort(__float2half_rn(v));
+}
+
+// The same where `on`, without a branch: many of them in a row keep going.
+template <class E>
+__device__ __forceinline__ void store_if(bool on, typename E::Storage* p, float v) {
+  if constexpr (E::kElem == FK_F32) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t@q st.global.f32 [%1], %2;\n\t}" ::"r"((int)on),
+                 "l"(p), "f"(v)
+                 : "memory");
+  } else {
+    const uint16_t h = E::kElem == FK_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t@q st.global.u16 [%1], %2;\n\t}" ::"r"((int)on),
+                 "l"(p), "h"(h)
+                 : "memory");
+  }
 }
 
 }  // namespace mx

@@ -100,21 +100,6 @@ __device__ __forceinline__ void mma_tf32(uint32_t tmem, uint64_t da, uint64_t db
       "l"(da), "l"(db), "r"(idesc), "r"(accumulate));
 }
 
-// kind::f16 with binary16 A and B, both K-major in shared memory, f32
-// accumulators, M = 128 rows, N columns (a multiple of 16, at most 256); an
-// instruction takes 16 of K (32 bytes of each row).
-__host__ __device__ constexpr uint32_t f16_idesc(uint32_t n, uint32_t m = 128) {
-  return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24);
-}
-
-__device__ __forceinline__ void mma_f16(uint32_t tmem, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem),
-      "l"(da), "l"(db), "r"(idesc), "r"(accumulate));
-}
-
 // The same with the A operand in tensor memory (128 lanes, a row a lane,
 // one 32-bit column a K element), B in shared memory.
 __device__ __forceinline__ void mma_tf32_ts(uint32_t tmem, uint32_t a_tmem, uint64_t db, uint32_t idesc,
@@ -123,6 +108,24 @@ __device__ __forceinline__ void mma_tf32_ts(uint32_t tmem, uint32_t a_tmem, uint
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(tmem),
+      "r"(a_tmem), "l"(db), "r"(idesc), "r"(accumulate));
+}
+
+// The instruction descriptor of kind::f16: f32 accumulators, binary16 A and
+// B, both K-major, N columns (a multiple of 16, at most 256), M = 128 rows;
+// an instruction takes 16 of K (32 bytes of each row).
+__host__ __device__ constexpr uint32_t f16_idesc(uint32_t n, uint32_t m = 128) {
+  return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+// kind::f16 with the A operand in tensor memory: a row a lane, two
+// neighbouring K elements a 32-bit column.
+__device__ __forceinline__ void mma_f16_ts(uint32_t tmem, uint32_t a_tmem, uint64_t db, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(tmem),
       "r"(a_tmem), "l"(db), "r"(idesc), "r"(accumulate));
 }
 

@@ -47,19 +47,28 @@ constexpr uint32_t kThreads = 32 * (12 + kWidenWarps);
 // Warps: 0..7 drain, then the widening ones, then one that loads inputs, one
 // for the MMAs, one that loads codes and one idle. The launch gives each of
 // the 640 threads 96 registers (61440 in all); the drain warps, with a
-// tile's sums, take 128 and the others 72 (256 x 128 + 384 x 72 = 60416).
-constexpr uint32_t kDrainRegs = 128, kOtherRegs = 72;
-__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kDrainRegs)); }
-__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs)); }
+// tile's sums, take 112 and the others 80 (256 x 112 + 384 x 80 = 59392), or
+// 144 and 64 (61440) for tiles of 192 tokens.
+template <int TN>
+__device__ __forceinline__ void drain_registers() {
+  if constexpr (TN > 96)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+  else
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+}
+template <int TN>
+__device__ __forceinline__ void other_registers() {
+  if constexpr (TN > 96)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  else
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+}
 constexpr uint32_t kMaxStages = 6;    // of inputs
+constexpr uint32_t kWide = 4;         // slabs of widened weights, 32 columns of tensor memory each
+constexpr uint32_t kCodes = 6;        // stages of codes (even: a stage stays one set's)
 constexpr uint32_t kDone = 8;         // slabs whose MMAs' end is told apart
 constexpr uint32_t kScaleSlots = 12;  // runs whose factors are held
 constexpr uint32_t kSmemBudget = 226 * 1024;
-// Stages of widened weights and of codes (even: a stage stays one set's):
-// what the widest tiles' inputs leave, else enough for two pairs of slabs a
-// set.
-__host__ __device__ constexpr uint32_t wide_stages(int n) { return n >= 256 ? 4 : 6; }
-__host__ __device__ constexpr uint32_t code_stages(int n) { return n >= 256 ? 2 : 6; }
 constexpr uint32_t kMaxEntries = 4096;
 
 // Status codes (first one wins), after the TF32 GEMMs'.
@@ -189,19 +198,18 @@ __device__ __forceinline__ uint32_t top_scale(const uint4& s) {
   return m;
 }
 
-// All but the inputs' stages: widened weights, codes, factors, each drain
-// warp's factors, barriers, and the alignment's slack.
-__host__ __device__ constexpr uint32_t fixed_bytes(int parts, int tn) {
-  return wide_stages(parts * tn) * kRows * 128 + code_stages(parts * tn) * kRows * 64 + kScaleSlots * kRows * 4 +
-         8 * (tn / 2) * 4 + 512 + 1024;
+// All but the inputs' stages: codes, factors, each drain warp's factors
+// and output places, barriers, and the alignment's slack.
+__host__ __device__ constexpr uint32_t fixed_bytes(int tn) {
+  return kCodes * kRows * 64 + kScaleSlots * kRows * 4 + 8 * (tn / 2) * 12 + 512 + 1024;
 }
 __host__ __device__ constexpr uint32_t stages_of(int parts, int tn) {
-  return (kSmemBudget - fixed_bytes(parts, tn)) / (uint32_t)(parts * tn * 128) < kMaxStages
-             ? (kSmemBudget - fixed_bytes(parts, tn)) / (uint32_t)(parts * tn * 128)
+  return (kSmemBudget - fixed_bytes(tn)) / (uint32_t)(parts * tn * 128) < kMaxStages
+             ? (kSmemBudget - fixed_bytes(tn)) / (uint32_t)(parts * tn * 128)
              : kMaxStages;
 }
 __host__ __device__ constexpr uint32_t smem_of(int parts, int tn) {
-  return fixed_bytes(parts, tn) + stages_of(parts, tn) * (uint32_t)(parts * tn * 128);
+  return fixed_bytes(tn) + stages_of(parts, tn) * (uint32_t)(parts * tn * 128);
 }
 
 template <class E, int PARTS, int TN>
@@ -209,15 +217,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     tile_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw, const Args a,
                 long long wait_cycles, int* __restrict__ err) {
   constexpr uint32_t N = PARTS * TN;  // the MMA's columns
-  constexpr uint32_t S = stages_of(PARTS, TN), kWide = wide_stages(N), kCodes = code_stages(N);
-  constexpr uint32_t kCols = 2 * N < 32 ? 32 : 2 * N;
+  constexpr uint32_t S = stages_of(PARTS, TN), kCols = 2 * N + 32 * kWide <= 256 ? 256 : 512;
+  static_assert(2 * N + 32 * kWide <= 512, "tensor memory: two runs' sums and the widened weights");
   constexpr uint32_t kHalf = TN / 2;  // a drain warp's tokens
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (an offset, so that the loads stay shared memory's)
   uint8_t* xs = smem;                            // [S][N rows][128 bytes]
-  uint8_t* ws = xs + S * N * 128;                // [kWide][128 rows][128 bytes]
-  uint8_t* raw = ws + kWide * kRows * 128;       // [kCodes][128 rows][64 bytes]
-  float* swb = reinterpret_cast<float*>(raw + kCodes * kRows * 64);  // [kScaleSlots][128]
+  uint8_t* raw = xs + S * N * 128;               // [kCodes][128 rows][64 bytes]
+  uint64_t* places = reinterpret_cast<uint64_t*>(raw + kCodes * kRows * 64);  // [8 drain warps][kHalf]
+  float* swb = reinterpret_cast<float*>(places + 8 * kHalf);         // [kScaleSlots][128]
   float* sxb = swb + kScaleSlots * kRows;                            // [8 drain warps][kHalf]
   uint64_t* bars = reinterpret_cast<uint64_t*>(sxb + 8 * kHalf);
   // full: a slab's inputs and widened weights; done: its MMAs; rfull and
@@ -282,12 +290,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto done_bar = [&](uint32_t j) { return &done[j % kDone]; };
 
   if (warp < 8) {
-    take_registers();
+    drain_registers<TN>();
     // Drain: warp w reads TMEM lanes 32 (w % 4).. (weight rows) of the
     // tokens of its half, adds each run's sums, times both factors, and
     // stores a token's 32 neighbouring outputs together.
     const uint32_t quarter = warp & 3, half = warp >> 2;
     float* mysx = sxb + warp * kHalf;
+    uint64_t* place = places + warp * kHalf;
     const uint32_t at = tmem + ((32 * quarter) << 16) + half * kHalf;
     uint32_t g = 0;  // runs so far
     bool ok = true;  // false: a wait ran out, the sums are not to be used (the status says so)
@@ -296,13 +305,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (uint32_t c = 0; c < kHalf; ++c) acc[c] = 0.0f;
       __syncwarp();
-      uint64_t place[(kHalf + 31) / 32];  // lane l: where tokens l, l + 32 of the half go
-#pragma unroll
-      for (uint32_t c = 0; c < kHalf; c += 32) {
-        const uint32_t in_tile = half * kHalf + c + lane, slot = o.slot0 + in_tile;
-        const bool live = c + lane < kHalf && in_tile < o.count;
-        const uint32_t p = live ? (a.perm ? __ldg(a.perm + slot) : slot) : 0;
-        place[c / 32] = (uint64_t)(p / a.k) * a.ldy + (uint64_t)(p % a.k) * a.n + o.row0 + 32 * quarter;
+      __syncwarp();
+      for (uint32_t c = lane; c < kHalf; c += 32) {
+        const uint32_t in_tile = half * kHalf + c, slot = o.slot0 + in_tile;
+        const uint32_t p = in_tile >= o.count ? 0 : a.perm ? __ldg(a.perm + slot) : slot;
+        place[c] = (uint64_t)(p / a.k) * a.ldy + (uint64_t)(p % a.k) * a.n + o.row0 + 32 * quarter;
       }
       for (uint32_t run = o.r0; run < o.r1; ++run, ++g) {
         __syncwarp();
@@ -368,23 +375,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       typename E::Storage* y = static_cast<typename E::Storage*>(a.y) + lane;
-      const bool live = o.row0 + 32 * quarter + lane < a.n;
+      // Tokens of this half; none where the lane's row is past the last.
+      const uint32_t count = o.row0 + 32 * quarter + lane < a.n ? o.count - min(o.count, half * kHalf) : 0;
 #pragma unroll
-      for (uint32_t c = 0; c < kHalf; ++c) {
-        const uint64_t to = __shfl_sync(0xffffffffu, place[c / 32], c % 32);
-        if (live && half * kHalf + c < o.count) mx::store<E>(y + to, acc[c]);
-      }
+      for (uint32_t c = 0; c < kHalf; ++c) mx::store_if<E>(c < count, y + place[c], acc[c]);
     }
   } else if (warp < 8 + kWidenWarps) {
-    give_registers();
-    // Widen: sets of four warps take pairs of slabs in turn, a thread a row:
-    // 64 bytes of codes to twice 128 bytes of binary16, where the 128-byte
-    // swizzle puts them (chunk c of row r at c ^ (r % 8); a codes' chunk at
-    // c ^ (r / 2 % 4)).
-    const uint32_t id = threadIdx.x - 256, row = id & 127, set = id >> 7, turn = row & 7;
+    other_registers<TN>();
+    // Widen: sets of four warps take pairs of slabs in turn, a thread a row
+    // (its TMEM lane): 64 bytes of codes (chunk c of row r at c ^ (r / 2 %
+    // 4), the 64-byte swizzle) to twice 32 columns of binary16 pairs.
+    const uint32_t id = threadIdx.x - 256, row = id & 127, set = id >> 7, turn4 = (row >> 1) & 3;
     const uint32_t nb = a.kk / mx::kBlock;
     const uint8_t* from = raw + row * 64;
-    uint8_t* to = ws + row * 128;
+    const uint32_t to = tmem + ((32 * (warp & 3)) << 16) + 2 * N;
     uint32_t i = 0, s = 0, q = 0, g = 0;  // slabs so far, their place in the ring, pairs, runs
     auto scales_of = [&](const Piece& p) {
       return a.scales + ((size_t)p.e * a.n + min(p.row0 + row, a.n - 1)) * nb;
@@ -399,15 +403,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (ok && more) {
       const Piece p = o;
       const uint8_t* prow = srow;
-      more = work.next(a, o);
-      if (more) srow = scales_of(o);
       for (uint32_t run = p.r0; ok && run < p.r1; ++run, ++g) {
         // A run's scales are loaded one run ahead, the next piece's first too.
         const uint4 sc = next;
-        if (run + 1 < p.r1)
+        if (run + 1 < p.r1) {
           next = load_scales(prow, (run + 1) * (kRun / mx::kBlock), nb);
-        else if (more)
+        } else if ((more = work.next(a, o))) {
+          srow = scales_of(o);
           next = load_scales(srow, o.r0 * (kRun / mx::kBlock), nb);
+        }
         const int ref = (int)top_scale(sc);
         if (set == 0) {
           // The factor back: 2^(ref - 127 - 12).
@@ -422,40 +426,39 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (uint32_t d = run * (kRun / kPairK); d < end; ++d, ++q) {
           const bool two = 2 * d + 1 < slabs;
           if (q % kSets == set) {
-            const uint32_t rs = q % kCodes, turn4 = (row >> 1) & 3, w = d % 4;
+            const uint32_t rs = q % kCodes, w = d % 4;
             const uint32_t four = w < 2 ? (w == 0 ? sc.x : sc.y) : (w == 2 ? sc.z : sc.w);  // the blocks' scales
             if (!(ok = wait(&rfull[rs], (q / kCodes) & 1, LT_TIMEOUT_CODES))) break;
-            uint4 codes[4];
 #pragma unroll
-            for (uint32_t c = 0; c < 4; ++c)
-              codes[c] = *reinterpret_cast<const uint4*>(from + rs * kRows * 64 + ((c ^ turn4) << 4));
-            // Both slabs' places are free once the slab before the second's last use is done.
-            const uint32_t before = i + 1 - kWide;
-            if (i + 1 >= kWide && !(ok = wait(done_bar(before), before / kDone & 1, LT_TIMEOUT_MMA))) break;
+            for (uint32_t h = 0; h < 2; ++h) {
+              if (h == 1 && !two) break;
+              uint32_t wide[32];
 #pragma unroll
-            for (uint32_t c = 0; c < 4; ++c) {
-              if (c == 2 && !two) break;
-              const uint32_t byte = (four >> (8 * c)) & 0xFFu;
-              const uint32_t by = byte == 255 ? 0x7E007E00u : half_power2((int)byte - ref + 12);
-              const uint32_t at = c < 2 ? s : s + 1 == kWide ? 0 : s + 1;
-              const uint32_t words[4] = {codes[c].x, codes[c].y, codes[c].z, codes[c].w};
+              for (uint32_t c = 0; c < 2; ++c) {
+                const uint4 v = *reinterpret_cast<const uint4*>(from + rs * kRows * 64 + (((2 * h + c) ^ turn4) << 4));
+                const uint32_t byte = (four >> (8 * (2 * h + c))) & 0xFFu;
+                const uint32_t by = byte == 255 ? 0x7E007E00u : half_power2((int)byte - ref + 12);
+                const uint32_t words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-              for (uint32_t v = 0; v < 4; ++v) {
-                uint32_t h[4];
-                mx::widen8_f16(words[v], h);
+                for (uint32_t u = 0; u < 4; ++u) {
+                  uint32_t f[4];
+                  mx::widen8_f16(words[u], f);
 #pragma unroll
-                for (int u = 0; u < 4; ++u) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[u]) : "r"(by));
-                *reinterpret_cast<uint4*>(to + at * kRows * 128 + (((c % 2 * 4 + v) ^ turn) << 4)) =
-                    make_uint4(h[0], h[1], h[2], h[3]);
+                  for (int e = 0; e < 4; ++e)
+                    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(wide[16 * c + 4 * u + e]) : "r"(f[e]), "r"(by));
+                }
               }
+              // Widened in registers while the columns were still in use.
+              const uint32_t before = i + h - kWide;
+              if (i + h >= kWide && !(ok = wait(done_bar(before), before / kDone & 1, LT_TIMEOUT_MMA))) break;
+              tmem_st32(to + 32 * (h == 0 ? s : s + 1 == kWide ? 0 : s + 1), wide);
+              tmem_wait_st();
+              fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(smem_u32(&full[(i + h) % kDone]));
             }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              mbar_arrive(smem_u32(&full[i % kDone]));
-              if (two) mbar_arrive(smem_u32(&full[(i + 1) % kDone]));
-              mbar_arrive(smem_u32(&rempty[rs]));
-            }
+            if (!ok) break;
+            if (lane == 0) mbar_arrive(smem_u32(&rempty[rs]));
           }
           i += two ? 2 : 1;
           s += two ? 2 : 1;
@@ -464,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-  give_registers();
+  other_registers<TN>();
   if (warp == kInputWarp && elect_one()) {
     // Inputs: a slab's N rows, the parts one below the other.
     uint32_t i = 0, s = 0;
@@ -498,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       wait1(&rfull[j % kCodes], (j / kCodes) & 1, LT_TIMEOUT_CODES);
   } else if (warp == kMmaWarp && elect_one()) {
     constexpr uint32_t idesc = f16_idesc(N);
-    const uint64_t wd0 = sw128_desc(smem_u32(ws)), xd0 = sw128_desc(smem_u32(xs));
+    const uint64_t xd0 = sw128_desc(smem_u32(xs));
     uint32_t i = 0, g = 0, s = 0, sw = 0;
     bool ok = true;
     while (ok && work.next(a, o))
@@ -510,10 +513,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!(ok = wait1(&full[i % kDone], i / kDone & 1, LT_TIMEOUT_INPUTS))) break;
           fence_after();
           // A K step of 16 is 32 bytes of each row: 2 in a descriptor's address.
-          const uint64_t wd = wd0 + sw * (kRows * 128 / 16), xd = xd0 + s * (N * 128 / 16);
+          const uint64_t xd = xd0 + s * (N * 128 / 16);
+          const uint32_t wa = tmem + 2 * N + 32 * sw;
 #pragma unroll
           for (uint32_t j = 0; j < kSlab / 16; ++j)
-            mma_f16(to, wd + 2 * j, xd + 2 * j, idesc, slab > 0 || j > 0 ? 1u : 0u);
+            mma_f16_ts(to, wa + 8 * j, xd + 2 * j, idesc, slab > 0 || j > 0 ? 1u : 0u);
           mma_commit(smem_u32(done_bar(i)));
           s = s + 1 == S ? 0 : s + 1;
           sw = sw + 1 == kWide ? 0 : sw + 1;
@@ -739,9 +743,17 @@ cudaError_t launch_all(const FkLinearMx& a, int sms, int* err, bool pdl, cudaStr
     tpre = reinterpret_cast<uint32_t*>(take(4 * (a.entries + 1)));
     perm = reinterpret_cast<uint32_t*>(take(4 * pairs));
   }
-  // Token tiles as wide as an expert's mean share asks for.
+  // The token tile that costs an expert's mean share least: a slab of a tile
+  // of N = PARTS tn columns takes the MMAs 2 N cycles, and the widening warps
+  // about 330 whatever N is.
   const uint64_t share = (pairs + a.entries - 1) / a.entries;
-  const uint32_t tn = share <= 16 ? 16 : share <= 32 ? 32 : share <= 64 ? 64 : 128;
+  uint32_t tn = 16;
+  uint64_t least = ~0ull;
+  const uint32_t widths[] = {16, 32, 64, 96, 192 / PARTS};
+  for (uint32_t w : widths) {
+    const uint64_t slab = 2 * PARTS * w > 330 ? 2 * PARTS * w : 330, cost = (share + w - 1) / w * (slab + w / 4);
+    if (cost < least) least = cost, tn = w;
+  }
   if (a.ids) {
     cudaError_t e = fk_launch_ex(group_kernel, dim3(1), dim3(1024), 0, s, pdl, a.ids, (uint32_t)pairs, a.entries, tn,
                                  off, tpre, perm);
@@ -771,10 +783,13 @@ cudaError_t launch_all(const FkLinearMx& a, int sms, int* err, bool pdl, cudaStr
   Args g = {a.scales, a.y, perm, off,   tpre,            sx,     part, landed, a.entries,
             a.n,      a.kk, a.k, a.ldy, (uint32_t)pairs, wtiles, runs};
   const uint32_t ctas = (uint32_t)grid;
-  if (tn == 16) return launch_tile<E, PARTS, 16>(a, g, parts, ctas, err, pdl, s);
-  if (tn == 32) return launch_tile<E, PARTS, 32>(a, g, parts, ctas, err, pdl, s);
-  if (tn == 64) return launch_tile<E, PARTS, 64>(a, g, parts, ctas, err, pdl, s);
-  return launch_tile<E, PARTS, 128>(a, g, parts, ctas, err, pdl, s);
+  switch (tn) {
+    case 16: return launch_tile<E, PARTS, 16>(a, g, parts, ctas, err, pdl, s);
+    case 32: return launch_tile<E, PARTS, 32>(a, g, parts, ctas, err, pdl, s);
+    case 64: return launch_tile<E, PARTS, 64>(a, g, parts, ctas, err, pdl, s);
+    case 96: return launch_tile<E, PARTS, 96>(a, g, parts, ctas, err, pdl, s);
+    default: return launch_tile<E, PARTS, 192 / PARTS>(a, g, parts, ctas, err, pdl, s);
+  }
 }
 
 }  // namespace
