@@ -47,19 +47,23 @@ constexpr uint32_t kThreads = 32 * (12 + kWidenWarps);
 // Warps: 0..7 drain, then the widening ones, then one that loads inputs, one
 // for the MMAs, one that loads codes and one idle. The launch gives each of
 // the 640 threads 96 registers (61440 in all); the drain warps, with a
-// tile's sums, take 112 and the others 80 (256 x 112 + 384 x 80 = 59392), or
-// 144 and 64 (61440) for tiles of 192 tokens.
+// tile's sums, take 112 and the others 80 (256 x 112 + 384 x 80 = 59392),
+// 128 and 72 (60416) for tiles of 128 tokens, 144 and 64 (61440) for 192.
 template <int TN>
 __device__ __forceinline__ void drain_registers() {
-  if constexpr (TN > 96)
+  if constexpr (TN > 128)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+  else if constexpr (TN > 96)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
   else
     asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
 }
 template <int TN>
 __device__ __forceinline__ void other_registers() {
-  if constexpr (TN > 96)
+  if constexpr (TN > 128)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  else if constexpr (TN > 96)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   else
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
 }
@@ -218,7 +222,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 long long wait_cycles, int* __restrict__ err) {
   constexpr uint32_t N = PARTS * TN;  // the MMA's columns
   constexpr uint32_t S = stages_of(PARTS, TN), kCols = 2 * N + 32 * kWide <= 256 ? 256 : 512;
-  static_assert(2 * N + 32 * kWide <= 512, "tensor memory: two runs' sums and the widened weights");
+  // Tensor memory: a run's sums, two where they fit, and the widened weights.
+  constexpr uint32_t kSums = 2 * N + 32 * kWide <= 512 ? 2 : 1;
+  static_assert(kSums * N + 32 * kWide <= 512, "tensor memory");
   constexpr uint32_t kHalf = TN / 2;  // a drain warp's tokens
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (an offset, so that the loads stay shared memory's)
@@ -320,9 +326,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         ok = ok && wait(&sfull[g % kScaleSlots], (g / kScaleSlots) & 1, LT_TIMEOUT_WIDEN);
         const float sw = swb[(g % kScaleSlots) * kRows + 32 * quarter + lane];
-        ok = ok && wait(&afull[g & 1], (g >> 1) & 1, LT_TIMEOUT_MMA);
+        ok = ok && wait(&afull[g % kSums], g / kSums & 1, LT_TIMEOUT_MMA);
         fence_after();
-        const uint32_t from = at + (g & 1) * N;
+        const uint32_t from = at + g % kSums * N;
         constexpr uint32_t kPiece = kHalf < 16 ? kHalf : 16;
 #pragma unroll
         for (uint32_t c = 0; c < kHalf; c += kPiece) {
@@ -340,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&aempty[g & 1]));
+        if (lane == 0) mbar_arrive(smem_u32(&aempty[g % kSums]));
       }
       if (o.r1 - o.r0 < a.runs) {
         // A part of a tile: its sums to the workspace, by CTA and by whether
@@ -388,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t id = threadIdx.x - 256, row = id & 127, set = id >> 7, turn4 = (row >> 1) & 3;
     const uint32_t nb = a.kk / mx::kBlock;
     const uint8_t* from = raw + row * 64;
-    const uint32_t to = tmem + ((32 * (warp & 3)) << 16) + 2 * N;
+    const uint32_t to = tmem + ((32 * (warp & 3)) << 16) + kSums * N;
     uint32_t i = 0, s = 0, q = 0, g = 0;  // slabs so far, their place in the ring, pairs, runs
     auto scales_of = [&](const Piece& p) {
       return a.scales + ((size_t)p.e * a.n + min(p.row0 + row, a.n - 1)) * nb;
@@ -506,15 +512,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     while (ok && work.next(a, o))
       for (uint32_t run = o.r0; ok && run < o.r1; ++run, ++g) {
-        if (g >= 2 && !(ok = wait1(&aempty[g & 1], ((g >> 1) - 1) & 1, LT_TIMEOUT_DRAIN))) break;
+        if (g >= kSums && !(ok = wait1(&aempty[g % kSums], (g / kSums - 1) & 1, LT_TIMEOUT_DRAIN))) break;
         fence_after();
-        const uint32_t to = tmem + (g & 1) * N, end = min(kRun / kSlab, slabs - run * (kRun / kSlab));
+        const uint32_t to = tmem + g % kSums * N, end = min(kRun / kSlab, slabs - run * (kRun / kSlab));
         for (uint32_t slab = 0; slab < end; ++slab, ++i) {
           if (!(ok = wait1(&full[i % kDone], i / kDone & 1, LT_TIMEOUT_INPUTS))) break;
           fence_after();
           // A K step of 16 is 32 bytes of each row: 2 in a descriptor's address.
           const uint64_t xd = xd0 + s * (N * 128 / 16);
-          const uint32_t wa = tmem + 2 * N + 32 * sw;
+          const uint32_t wa = tmem + kSums * N + 32 * sw;
 #pragma unroll
           for (uint32_t j = 0; j < kSlab / 16; ++j)
             mma_f16_ts(to, wa + 8 * j, xd + 2 * j, idesc, slab > 0 || j > 0 ? 1u : 0u);
@@ -522,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           s = s + 1 == S ? 0 : s + 1;
           sw = sw + 1 == kWide ? 0 : sw + 1;
         }
-        if (ok) mma_commit(smem_u32(&afull[g & 1]));
+        if (ok) mma_commit(smem_u32(&afull[g % kSums]));
       }
     // Every MMA issued has finished before the CTA frees its tensor memory.
     mma_commit(smem_u32(fin));
@@ -749,7 +755,8 @@ cudaError_t launch_all(const FkLinearMx& a, int sms, int* err, bool pdl, cudaStr
   const uint64_t share = (pairs + a.entries - 1) / a.entries;
   uint32_t tn = 16;
   uint64_t least = ~0ull;
-  const uint32_t widths[] = {16, 32, 64, 96, 192 / PARTS};
+  constexpr uint32_t kWidest = PARTS == 2 ? 128 : 192;
+  const uint32_t widths[] = {16, 32, 64, 96, kWidest};
   for (uint32_t w : widths) {
     const uint64_t slab = 2 * PARTS * w > 330 ? 2 * PARTS * w : 330, cost = (share + w - 1) / w * (slab + w / 4);
     if (cost < least) least = cost, tn = w;
@@ -788,7 +795,7 @@ cudaError_t launch_all(const FkLinearMx& a, int sms, int* err, bool pdl, cudaStr
     case 32: return launch_tile<E, PARTS, 32>(a, g, parts, ctas, err, pdl, s);
     case 64: return launch_tile<E, PARTS, 64>(a, g, parts, ctas, err, pdl, s);
     case 96: return launch_tile<E, PARTS, 96>(a, g, parts, ctas, err, pdl, s);
-    default: return launch_tile<E, PARTS, 192 / PARTS>(a, g, parts, ctas, err, pdl, s);
+    default: return launch_tile<E, PARTS, kWidest>(a, g, parts, ctas, err, pdl, s);
   }
 }
 
