@@ -82,7 +82,7 @@ def lib() -> ctypes.CDLL:
                                           ctypes.POINTER(u32)]),
             "fkc_kernel_find": (i32, [ctypes.c_char_p, u64, ctypes.POINTER(i32)]),
             "fkc_fnv1a64": (u64, [vp, sz]),
-            "fkc_launch": (i32, [vp, i32, vp, sz, pvp, i32]),
+            "fkc_launch": (i32, [vp, i32, vp, sz, vp, i32]),
             "fkc_linear_mxfp4_work": (i32, [u32, u32, u32, u32, u32, ctypes.POINTER(sz)]),
             "fkc_capture_begin": (i32, [vp]),
             "fkc_capture_end": (i32, [vp, pvp]),
@@ -383,8 +383,12 @@ class Context:
         if e is None:
             raise Refused(FKC_ERR_ARGUMENT, f"The target has no kernel {kernel}.")
         raw = e.pack(params)
-        ptrs = (ctypes.c_void_p * len(bufs))(*[b.ptr if isinstance(b, DeviceBuffer) else int(b) for b in bufs])
-        check(lib().fkc_launch(self.handle, e.id, raw or None, len(raw), ptrs, len(bufs)))
+        # The addresses as the array of pointers that fkc_launch reads.
+        ptrs = struct.pack(f"{len(bufs)}P", *[b if b.__class__ is int else b.ptr if isinstance(b, DeviceBuffer) else int(b)
+                                              for b in bufs])
+        rc = _lib.fkc_launch(self.handle, e.id, raw or None, len(raw), ptrs, len(bufs))
+        if rc:
+            check(rc)
 
     def capture_begin(self) -> None:
         check(lib().fkc_capture_begin(self.handle))

@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(128) route_grouped_kernel(FkRouteGrouped a) {
   }
   if (a.sigmoid) {
 #pragma unroll
-    for (int t = 0; t < T; ++t) s[t] = __fdiv_rn(1.0f, __fadd_rn(1.0f, exp_rounded(-s[t])));
+    for (int t = 0; t < T; ++t) s[t] = __frcp_rn(__fadd_rn(1.0f, exp_rounded(-s[t])));
   } else {
     float top = -INFINITY;
 #pragma unroll
@@ -84,30 +84,48 @@ __global__ void __launch_bounds__(128) route_grouped_kernel(FkRouteGrouped a) {
     const uint32_t i = lane + 32 * t;
     key[t] = i < a.n ? key_of(a.bias ? __fadd_rn(s[t], __ldg(a.bias + i)) : s[t]) : 0u;
   }
-  const uint32_t per = a.n / a.groups;
   if (a.top_groups < a.groups) {
+    const uint32_t per = a.n / a.groups;
     uint32_t worth = 0;  // lane g: group g's worth
-    for (uint32_t g = 0; g < a.groups; ++g) {
-      uint32_t k1 = 0, k2 = 0;  // this lane's largest two of the group
-#pragma unroll
-      for (int t = 0; t < T; ++t) {
-        const uint32_t i = lane + 32 * t;
-        if (i / per == g) {
-          if (key[t] > k1)
-            k2 = k1, k1 = key[t];
-          else if (key[t] > k2)
-            k2 = key[t];
-        }
-      }
-      const uint32_t m1 = __reduce_max_sync(kAll, k1);
-      uint32_t w = m1;
+    // From each lane's largest two keys of group g.
+    auto close = [&](uint32_t g, uint32_t k1, uint32_t k2) {
+      uint32_t w = __reduce_max_sync(kAll, k1);
       if (a.group_by == 2 && per > 1) {
         // The largest but one: the first lane with the largest offers its second.
-        const uint32_t has = __ballot_sync(kAll, k1 == m1);
+        const uint32_t has = __ballot_sync(kAll, k1 == w);
         const uint32_t m2 = __reduce_max_sync(kAll, lane == (uint32_t)__ffs(has) - 1 ? k2 : k1);
-        w = key_of(__fadd_rn(of_key(m1), of_key(m2)));
+        w = key_of(__fadd_rn(of_key(w), of_key(m2)));
       }
       if (lane == g) worth = w;
+    };
+    uint32_t group[T];  // the group of each of the lane's experts
+    if (per % 32 == 0) {  // a group is whole turns of the lanes: one pass
+      uint32_t g = 0, left = per / 32, k1 = 0, k2 = 0;
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        group[t] = g;
+        if (g < a.groups) {
+          k2 = key[t] > k1 ? k1 : max(k2, key[t]);
+          k1 = max(k1, key[t]);
+          if (--left == 0) {
+            close(g, k1, k2);
+            ++g, left = per / 32, k1 = k2 = 0;
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < T; ++t) group[t] = (lane + 32 * t) / per;
+      for (uint32_t g = 0; g < a.groups; ++g) {
+        uint32_t k1 = 0, k2 = 0;
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+          const uint32_t k = group[t] == g ? key[t] : 0u;
+          k2 = k > k1 ? k1 : max(k2, k);
+          k1 = max(k1, k);
+        }
+        close(g, k1, k2);
+      }
     }
     uint32_t kept = 0;
     for (uint32_t j = 0; j < a.top_groups; ++j) {
@@ -118,8 +136,7 @@ __global__ void __launch_bounds__(128) route_grouped_kernel(FkRouteGrouped a) {
     }
 #pragma unroll
     for (int t = 0; t < T; ++t) {
-      const uint32_t i = lane + 32 * t;
-      if (i < a.n && !((kept >> (i / per)) & 1u)) key[t] = 0;
+      if (group[t] < a.groups && !((kept >> group[t]) & 1u)) key[t] = 0;
     }
   }
   // k rounds: the largest key, the lowest index among its holders.
