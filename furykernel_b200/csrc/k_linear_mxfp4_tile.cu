@@ -40,36 +40,32 @@ constexpr uint32_t kRows = 128;   // weight rows a tile: the MMA's M, TMEM lanes
 constexpr uint32_t kSlab = 64;    // K of a stage: 128 bytes of binary16
 constexpr uint32_t kRun = 512;    // K of a run
 constexpr uint32_t kPairK = 128;  // K of a stage of codes: 64 bytes, two slabs
-constexpr uint32_t kSets = 2;                       // of four widening warps, which take slabs in turn
+constexpr uint32_t kSets = 3;                       // of four widening warps, which take slabs in turn
 constexpr uint32_t kWidenWarps = 4 * kSets;
 constexpr uint32_t kInputWarp = 8 + kWidenWarps, kMmaWarp = kInputWarp + 1, kCodeWarp = kInputWarp + 2;
 constexpr uint32_t kThreads = 32 * (12 + kWidenWarps);
 // Warps: 0..7 drain, then the widening ones, then one that loads inputs, one
 // for the MMAs, one that loads codes and one idle. The launch gives each of
-// the 640 threads 96 registers (61440 in all); the drain warps, with a
-// tile's sums, take 112 and the others 80 (256 x 112 + 384 x 80 = 59392),
-// 128 and 72 (60416) for tiles of 128 tokens, 144 and 64 (61440) for 192.
+// the 768 threads 80 registers (61440 in all); the drain warps, with a
+// tile's sums, take 112 and the others 64 (256 x 112 + 512 x 64 = 61440), or
+// 128 and 56 (61440) for tiles of 128 and more tokens.
 template <int TN>
 __device__ __forceinline__ void drain_registers() {
-  if constexpr (TN > 128)
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
-  else if constexpr (TN > 96)
+  if constexpr (TN > 96)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
   else
     asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
 }
 template <int TN>
 __device__ __forceinline__ void other_registers() {
-  if constexpr (TN > 128)
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-  else if constexpr (TN > 96)
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  if constexpr (TN > 96)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   else
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
 }
 constexpr uint32_t kMaxStages = 6;    // of inputs
-constexpr uint32_t kWide = 4;         // slabs of widened weights, 32 columns of tensor memory each
-constexpr uint32_t kCodes = 6;        // stages of codes (even: a stage stays one set's)
+constexpr uint32_t kWide = 6;         // slabs of widened weights, 32 columns of tensor memory each
+constexpr uint32_t kCodes = 6;        // stages of codes (a multiple of the sets: a stage stays one set's)
 constexpr uint32_t kDone = 8;         // slabs whose MMAs' end is told apart
 constexpr uint32_t kScaleSlots = 12;  // runs whose factors are held
 constexpr uint32_t kSmemBudget = 226 * 1024;
@@ -329,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = ok && wait(&afull[g % kSums], g / kSums & 1, LT_TIMEOUT_MMA);
         fence_after();
         const uint32_t from = at + g % kSums * N;
-        constexpr uint32_t kPiece = kHalf < 16 ? kHalf : 16;
+        constexpr uint32_t kPiece = kHalf % 16 ? 8 : 16;
 #pragma unroll
         for (uint32_t c = 0; c < kHalf; c += kPiece) {
           uint32_t r0[kPiece], r1[kPiece];
@@ -353,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // the tile starts here; the last of the tile's CTAs to do so adds
         // them all, in the CTAs' order.
         constexpr size_t stride = (size_t)TN * kRows;
-        constexpr uint32_t kAtOnce = kHalf < 16 ? kHalf : 16;
+        constexpr uint32_t kAtOnce = kHalf % 16 ? 8 : 16;
         const uint32_t first = o.tile * a.runs;
         const uint32_t c0 = work.owner(first), c1 = work.owner(first + a.runs - 1);
         const size_t mine = (size_t)(half * kHalf) * kRows + 32 * quarter + lane;
@@ -438,26 +434,30 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h) {
               if (h == 1 && !two) break;
-              uint32_t wide[32];
+              const uint32_t at = to + 32 * (h == 0 ? s : s + 1 == kWide ? 0 : s + 1);
 #pragma unroll
               for (uint32_t c = 0; c < 2; ++c) {
                 const uint4 v = *reinterpret_cast<const uint4*>(from + rs * kRows * 64 + (((2 * h + c) ^ turn4) << 4));
                 const uint32_t byte = (four >> (8 * (2 * h + c))) & 0xFFu;
                 const uint32_t by = byte == 255 ? 0x7E007E00u : half_power2((int)byte - ref + 12);
                 const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+                uint32_t wide[16];
 #pragma unroll
                 for (uint32_t u = 0; u < 4; ++u) {
                   uint32_t f[4];
                   mx::widen8_f16(words[u], f);
 #pragma unroll
                   for (int e = 0; e < 4; ++e)
-                    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(wide[16 * c + 4 * u + e]) : "r"(f[e]), "r"(by));
+                    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(wide[4 * u + e]) : "r"(f[e]), "r"(by));
                 }
+                // Half a slab is widened in registers while its columns may still be in use.
+                if (c == 0 && i + h >= kWide) {
+                  const uint32_t before = i + h - kWide;
+                  if (!(ok = wait(done_bar(before), before / kDone & 1, LT_TIMEOUT_MMA))) break;
+                }
+                tmem_st16(at + 16 * c, wide);
               }
-              // Widened in registers while the columns were still in use.
-              const uint32_t before = i + h - kWide;
-              if (i + h >= kWide && !(ok = wait(done_bar(before), before / kDone & 1, LT_TIMEOUT_MMA))) break;
-              tmem_st32(to + 32 * (h == 0 ? s : s + 1 == kWide ? 0 : s + 1), wide);
+              if (!ok) break;
               tmem_wait_st();
               fence_before();
               __syncwarp();
@@ -552,7 +552,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // column of a tile is computed by itself.
 __global__ void __launch_bounds__(1024) group_kernel(const uint32_t* __restrict__ ids, uint32_t pairs,
                                                      uint32_t entries, uint32_t tn, uint32_t* __restrict__ off,
-                                                     uint32_t* __restrict__ tpre, uint32_t* __restrict__ perm) {
+                                                     uint32_t* __restrict__ tpre, uint32_t* __restrict__ perm,
+                                                     uint32_t* __restrict__ slot_of) {
   __shared__ uint32_t count[kMaxEntries];
   __shared__ uint32_t sums[2][32];
   __shared__ uint32_t rest;
@@ -561,10 +562,26 @@ __global__ void __launch_bounds__(1024) group_kernel(const uint32_t* __restrict_
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   for (uint32_t e = tid; e < kMaxEntries; e += 1024) count[e] = 0;
   __syncthreads();
-  for (uint32_t p = tid; p < pairs; p += 1024) {
-    const uint32_t e = __ldg(ids + p);
+  // Four ids a load, 16 in flight; the last few singly.
+  auto each = [&](auto&& take) {
+    const uint32_t fours = pairs / 4;
+    for (uint32_t q0 = tid; q0 < fours; q0 += 4096) {
+      uint4 v[4];
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u)
+        if (q0 + 1024 * u < fours) v[u] = __ldg(reinterpret_cast<const uint4*>(ids) + q0 + 1024 * u);
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u)
+        if (q0 + 1024 * u < fours) {
+          const uint32_t p = 4 * (q0 + 1024 * u);
+          take(p, v[u].x), take(p + 1, v[u].y), take(p + 2, v[u].z), take(p + 3, v[u].w);
+        }
+    }
+    if (4 * fours + tid < pairs) take(4 * fours + tid, __ldg(ids + 4 * fours + tid));
+  };
+  each([&](uint32_t, uint32_t e) {
     if (e < entries) atomicAdd(&count[e], 1u);
-  }
+  });
   __syncthreads();
   // Thread t has experts 4t .. 4t + 3: exclusive sums of their counts and tiles.
   uint32_t c[4], slots = 0, tiles = 0;
@@ -607,10 +624,11 @@ __global__ void __launch_bounds__(1024) group_kernel(const uint32_t* __restrict_
     rest = s;
   }
   __syncthreads();
-  for (uint32_t p = tid; p < pairs; p += 1024) {
-    const uint32_t e = __ldg(ids + p);
-    perm[e < entries ? atomicAdd(&count[e], 1u) : atomicAdd(&rest, 1u)] = p;
-  }
+  each([&](uint32_t p, uint32_t e) {
+    const uint32_t slot = e < entries ? atomicAdd(&count[e], 1u) : atomicAdd(&rest, 1u);
+    perm[slot] = p;
+    slot_of[p] = slot;
+  });
 }
 
 // ---------------------------------------------------------------------------
@@ -621,14 +639,15 @@ struct SplitArgs {
   void* y;
   uint16_t* parts;  // [PARTS][slots][kk]
   float* sx;        // [runs][slots]
-  const uint32_t* perm;
+  const uint32_t* slot_of;  // pair -> slot, or null: the identity
   const uint32_t* off;
   uint32_t* landed;  // [grid] set to 0
   uint32_t entries, n, kk, k, ldx, ldy, slots, runs, grid;
   bool per_rank;
 };
 
-// A warp a (slot, run): 512 inputs, 16 a lane.
+// A warp a (row or pair with an input of its own, run): 512 inputs, 16 a
+// lane, to the slots of all the pairs that take them.
 template <class E, int PARTS>
 __global__ void __launch_bounds__(256) split_kernel(SplitArgs a) {
   grid_wait();
@@ -636,17 +655,11 @@ __global__ void __launch_bounds__(256) split_kernel(SplitArgs a) {
   const uint32_t lane = threadIdx.x & 31;
   if (blockIdx.x == 0)
     for (uint32_t c = threadIdx.x; c < a.grid; c += 256) a.landed[c] = 0;
+  const uint32_t copies = a.per_rank ? 1 : a.k;
   const uint64_t unit = blockIdx.x * 8ull + (threadIdx.x >> 5);
-  if (unit >= (uint64_t)a.slots * a.runs) return;
-  const uint32_t slot = (uint32_t)(unit / a.runs), run = (uint32_t)(unit % a.runs);
-  const uint32_t p = a.perm ? __ldg(a.perm + slot) : slot;
-  const uint32_t r = p / a.k, j = p % a.k;
-  if (a.off && slot >= __ldg(a.off + a.entries)) {  // a pair without an expert
-    if (run == 0)
-      for (uint32_t c = lane; c < a.n; c += 32)
-        mx::store<E>(static_cast<typename E::Storage*>(a.y) + (size_t)r * a.ldy + (size_t)j * a.n + c, 0.0f);
-    return;
-  }
+  if (unit >= (uint64_t)(a.slots / copies) * a.runs) return;
+  const uint32_t first = (uint32_t)(unit / a.runs) * copies, run = (uint32_t)(unit % a.runs);  // the first pair
+  const uint32_t r = first / a.k, j = first % a.k;
   const typename E::Storage* x =
       static_cast<const typename E::Storage*>(a.x) + (size_t)r * a.ldx + (a.per_rank ? (size_t)j * a.kk : 0);
   const bool wide = ((uintptr_t)x & 15) == 0;
@@ -664,18 +677,28 @@ __global__ void __launch_bounds__(256) split_kernel(SplitArgs a) {
   top = __reduce_max_sync(0xffffffffu, top);
   const int up = mx::input_shift<E>(top);
   const float by = mx::scale_value((uint32_t)(127 + up));
+  uint32_t lo[2][4], hi[2][4];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint32_t c = run * kRun + 256 * h + 8 * lane;
-    if (c >= a.kk) continue;
-    uint32_t lo[4], hi[4];
-    mx::split8<PARTS == 2>(v[h], by, hi, lo);
-    uint16_t* to = a.parts + (size_t)slot * a.kk + c;
-    *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    if constexpr (PARTS == 2)
-      *reinterpret_cast<uint4*>(to + (size_t)a.slots * a.kk) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  for (int h = 0; h < 2; ++h) mx::split8<PARTS == 2>(v[h], by, hi[h], lo[h]);
+  for (uint32_t q = 0; q < copies; ++q) {
+    const uint32_t slot = a.slot_of ? __ldg(a.slot_of + first + q) : first + q;
+    if (a.off && slot >= __ldg(a.off + a.entries)) {  // a pair without an expert: zeros
+      if (run == 0)
+        for (uint32_t c = lane; c < a.n; c += 32)
+          mx::store<E>(static_cast<typename E::Storage*>(a.y) + (size_t)r * a.ldy + (size_t)(j + q) * a.n + c, 0.0f);
+      continue;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t c = run * kRun + 256 * h + 8 * lane;
+      if (c >= a.kk) continue;
+      uint16_t* to = a.parts + (size_t)slot * a.kk + c;
+      *reinterpret_cast<uint4*>(to) = make_uint4(hi[h][0], hi[h][1], hi[h][2], hi[h][3]);
+      if constexpr (PARTS == 2)
+        *reinterpret_cast<uint4*>(to + (size_t)a.slots * a.kk) = make_uint4(lo[h][0], lo[h][1], lo[h][2], lo[h][3]);
+    }
+    if (lane == 0) a.sx[(size_t)run * a.slots + slot] = mx::scale_value((uint32_t)(127 - up));
   }
-  if (lane == 0) a.sx[(size_t)run * a.slots + slot] = mx::scale_value((uint32_t)(127 - up));
 }
 
 }  // namespace lt
@@ -744,26 +767,28 @@ cudaError_t launch_all(const FkLinearMx& a, int sms, int* err, bool pdl, cudaStr
   uint32_t* off = nullptr;
   uint32_t* tpre = nullptr;
   uint32_t* perm = nullptr;
+  uint32_t* slot_of = nullptr;
   if (a.ids) {
     off = reinterpret_cast<uint32_t*>(take(4 * (a.entries + 1)));
     tpre = reinterpret_cast<uint32_t*>(take(4 * (a.entries + 1)));
     perm = reinterpret_cast<uint32_t*>(take(4 * pairs));
+    slot_of = reinterpret_cast<uint32_t*>(take(4 * pairs));
   }
   // The token tile that costs an expert's mean share least: a slab of a tile
   // of N = PARTS tn columns takes the MMAs 2 N cycles, and the widening warps
-  // about 330 whatever N is.
+  // about 250 whatever N is.
   const uint64_t share = (pairs + a.entries - 1) / a.entries;
   uint32_t tn = 16;
   uint64_t least = ~0ull;
-  constexpr uint32_t kWidest = PARTS == 2 ? 128 : 192;
-  const uint32_t widths[] = {16, 32, 64, 96, kWidest};
+  constexpr uint32_t kWidest = PARTS == 2 ? 128 : 160;
+  const uint32_t widths[] = {16, 32, 64, 160 / PARTS, kWidest};
   for (uint32_t w : widths) {
-    const uint64_t slab = 2 * PARTS * w > 330 ? 2 * PARTS * w : 330, cost = (share + w - 1) / w * (slab + w / 4);
+    const uint64_t slab = 2 * PARTS * w > 250 ? 2 * PARTS * w : 250, cost = (share + w - 1) / w * (slab + w / 4);
     if (cost < least) least = cost, tn = w;
   }
   if (a.ids) {
     cudaError_t e = fk_launch_ex(group_kernel, dim3(1), dim3(1024), 0, s, pdl, a.ids, (uint32_t)pairs, a.entries, tn,
-                                 off, tpre, perm);
+                                 off, tpre, perm, slot_of);
     if (e != cudaSuccess) return e;
   }
   // A CTA an SM, each an equal share of the tiles' runs, where the parts of
@@ -782,9 +807,9 @@ cudaError_t launch_all(const FkLinearMx& a, int sms, int* err, bool pdl, cudaStr
     grid = split;
     part = reinterpret_cast<float*>(at);
   }
-  SplitArgs sp = {a.x,    a.y,   parts, sx,    perm,  off,   landed,          a.entries, a.n,
+  SplitArgs sp = {a.x,    a.y,   parts, sx,    slot_of, off, landed,          a.entries, a.n,
                   a.kk,   a.k,   a.ldx, a.ldy, (uint32_t)pairs, runs, (uint32_t)grid,  a.per_rank};
-  const uint64_t blocks = (pairs * runs + 7) / 8;
+  const uint64_t blocks = (pairs / (a.per_rank ? 1 : a.k) * runs + 7) / 8;
   cudaError_t e = fk_launch_ex(split_kernel<E, PARTS>, dim3((uint32_t)blocks), dim3(256), 0, s, pdl, sp);
   if (e != cudaSuccess) return e;
   Args g = {a.scales, a.y, perm, off,   tpre,            sx,     part, landed, a.entries,
@@ -794,7 +819,7 @@ cudaError_t launch_all(const FkLinearMx& a, int sms, int* err, bool pdl, cudaStr
     case 16: return launch_tile<E, PARTS, 16>(a, g, parts, ctas, err, pdl, s);
     case 32: return launch_tile<E, PARTS, 32>(a, g, parts, ctas, err, pdl, s);
     case 64: return launch_tile<E, PARTS, 64>(a, g, parts, ctas, err, pdl, s);
-    case 96: return launch_tile<E, PARTS, 96>(a, g, parts, ctas, err, pdl, s);
+    case 160 / PARTS: return launch_tile<E, PARTS, 160 / PARTS>(a, g, parts, ctas, err, pdl, s);
     default: return launch_tile<E, PARTS, kWidest>(a, g, parts, ctas, err, pdl, s);
   }
 }

@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(256) quant_kernel(const typename E::Storage* _
 // A thread four codes at a time, so that a warp's stores of f32 are whole
 // lines (eight a thread, in two stores, left half of each sector to the other).
 template <class E>
-__global__ void __launch_bounds__(256) widen_kernel(const uint16_t* __restrict__ codes,
+__global__ void __launch_bounds__(256) widen_kernel(const uint32_t* __restrict__ codes,
                                                     const uint8_t* __restrict__ scales, uint64_t rows, uint32_t k,
                                                     uint32_t ldy, typename E::Storage* __restrict__ y) {
   grid_wait();
@@ -103,10 +103,10 @@ __global__ void __launch_bounds__(256) widen_kernel(const uint16_t* __restrict__
   const uint64_t total = rows * quarters, stride = (uint64_t)gridDim.x * blockDim.x;
   const bool aligned = (uint64_t)ldy * sizeof(typename E::Storage) % 16 == 0, few = total < 0xFFFFFFFFull;
   auto put = [&](uint64_t at, uint32_t w, uint32_t s) {
-    uint32_t d[4];
+    uint32_t d[4];  // of the word's eight, this thread's four
     widen8_f16(w, d);
     const float f = scale_value(s);
-    const float2 a = F16::widen2(d[0]), b = F16::widen2(d[1]);
+    const float2 a = F16::widen2(at & 1 ? d[2] : d[0]), b = F16::widen2(at & 1 ? d[3] : d[1]);
     const float v[4] = {__fmul_rn(a.x, f), __fmul_rn(a.y, f), __fmul_rn(b.x, f), __fmul_rn(b.y, f)};
     typename E::Storage* to = y + place_of(at, 4, quarters, ldy, few);
     if (!aligned) {
@@ -126,13 +126,13 @@ __global__ void __launch_bounds__(256) widen_kernel(const uint16_t* __restrict__
     uint32_t w[kAhead], s[kAhead];
 #pragma unroll
     for (uint32_t u = 0; u < kAhead; ++u) {
-      w[u] = __ldg(codes + at + u * stride);
+      w[u] = __ldg(codes + ((at + u * stride) >> 1));
       s[u] = __ldg(scales + ((at + u * stride) >> 3));
     }
 #pragma unroll
     for (uint32_t u = 0; u < kAhead; ++u) put(at + u * stride, w[u], s[u]);
   }
-  for (; at < total; at += stride) put(at, __ldg(codes + at), __ldg(scales + (at >> 3)));
+  for (; at < total; at += stride) put(at, __ldg(codes + (at >> 1)), __ldg(scales + (at >> 3)));
 }
 
 // `a_sm` blocks an SM at most: 4 of the quantisation (1024 threads, 128 bytes
@@ -163,7 +163,7 @@ cudaError_t fk_launch_widen_mxfp4(const uint8_t* codes, const uint8_t* scales, u
   if (k % fk::mx::kBlock != 0 || ldy < k) return cudaErrorInvalidValue;
 #define FK_CALL(E)                                                                                      \
   fk_launch_ex(fk::mx::widen_kernel<E>, dim3(fk::mx::grid_for(rows * (k / 4), 64)), dim3(256), 0, s, pdl,   \
-               reinterpret_cast<const uint16_t*>(codes), scales, rows, k, ldy, static_cast<E::Storage*>(y))
+               reinterpret_cast<const uint32_t*>(codes), scales, rows, k, ldy, static_cast<E::Storage*>(y))
   return FK_BY_ELEM(e, FK_CALL);
 #undef FK_CALL
 }
