@@ -63,10 +63,10 @@ __device__ __forceinline__ void other_registers() {
   else
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
 }
-constexpr uint32_t kMaxStages = 6;    // of inputs
+constexpr uint32_t kMaxStages = 16;   // of inputs: a load takes 1000 to 3000 cycles to land
 constexpr uint32_t kWide = 6;         // slabs of widened weights, 32 columns of tensor memory each
 constexpr uint32_t kCodes = 6;        // stages of codes (a multiple of the sets: a stage stays one set's)
-constexpr uint32_t kDone = 8;         // slabs whose MMAs' end is told apart
+constexpr uint32_t kDone = 32;        // slabs whose MMAs' end is told apart
 constexpr uint32_t kScaleSlots = 12;  // runs whose factors are held
 constexpr uint32_t kSmemBudget = 226 * 1024;
 constexpr uint32_t kMaxEntries = 4096;
@@ -201,7 +201,7 @@ __device__ __forceinline__ uint32_t top_scale(const uint4& s) {
 // All but the inputs' stages: codes, factors, each drain warp's factors
 // and output places, barriers, and the alignment's slack.
 __host__ __device__ constexpr uint32_t fixed_bytes(int tn) {
-  return kCodes * kRows * 64 + kScaleSlots * kRows * 4 + 8 * (tn / 2) * 12 + 512 + 1024;
+  return kCodes * kRows * 64 + kScaleSlots * kRows * 4 + 8 * (tn / 2) * 12 + 1024 + 1024;
 }
 __host__ __device__ constexpr uint32_t stages_of(int parts, int tn) {
   return (kSmemBudget - fixed_bytes(tn)) / (uint32_t)(parts * tn * 128) < kMaxStages
