@@ -39,16 +39,16 @@ using namespace tc;
 constexpr uint32_t kRows = 128;   // weight rows a tile: the MMA's M, TMEM lanes
 constexpr uint32_t kSlab = 64;    // K of a stage: 128 bytes of binary16
 constexpr uint32_t kRun = 512;    // K of a run
-constexpr uint32_t kPairK = 128;  // K of a stage of codes: 64 bytes, two slabs
-constexpr uint32_t kSets = 3;                       // of four widening warps, which take slabs in turn
+constexpr uint32_t kHalfK = 256;  // K of a stage of codes: 128 bytes, half a run
+constexpr uint32_t kSets = 2;                       // of four widening warps, each a half of every run
 constexpr uint32_t kWidenWarps = 4 * kSets;
 constexpr uint32_t kInputWarp = 8 + kWidenWarps, kMmaWarp = kInputWarp + 1, kCodeWarp = kInputWarp + 2;
 constexpr uint32_t kThreads = 32 * (12 + kWidenWarps);
 // Warps: 0..7 drain, then the widening ones, then one that loads inputs, one
 // for the MMAs, one that loads codes and one idle. The launch gives each of
-// the 768 threads 80 registers (61440 in all); the drain warps, with a
-// tile's sums, take 112 and the others 64 (256 x 112 + 512 x 64 = 61440), or
-// 128 and 56 (61440) for tiles of 128 and more tokens.
+// the 640 threads 96 registers (61440 in all); the drain warps, with a
+// tile's sums, take 112 and the others 80 (256 x 112 + 384 x 80 = 59392), or
+// 128 and 72 (60416) for tiles of 128 and more tokens.
 template <int TN>
 __device__ __forceinline__ void drain_registers() {
   if constexpr (TN > 96)
@@ -59,13 +59,12 @@ __device__ __forceinline__ void drain_registers() {
 template <int TN>
 __device__ __forceinline__ void other_registers() {
   if constexpr (TN > 96)
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   else
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
 }
 constexpr uint32_t kMaxStages = 16;   // of inputs: a load takes 1000 to 3000 cycles to land
-constexpr uint32_t kWide = 6;         // slabs of widened weights, 32 columns of tensor memory each
-constexpr uint32_t kCodes = 6;        // stages of codes (a multiple of the sets: a stage stays one set's)
+constexpr uint32_t kCodes = 4;        // stages of codes
 constexpr uint32_t kDone = 32;        // slabs whose MMAs' end is told apart
 constexpr uint32_t kScaleSlots = 12;  // runs whose factors are held
 constexpr uint32_t kSmemBudget = 226 * 1024;
@@ -151,12 +150,6 @@ struct Work {
   }
 };
 
-// Binary16 2^j as a pair, 0 below the type's range.
-__device__ __forceinline__ uint32_t half_power2(int j) {
-  const uint32_t h = j >= -14 ? (uint32_t)(j + 15) << 10 : j >= -24 ? 1u << (j + 24) : 0u;
-  return h | h << 16;
-}
-
 // A row's 16 scale bytes of a run, from block b0 on; past the row's nb: 0.
 // Rows start on multiples of nb bytes.
 __device__ __forceinline__ uint4 load_scales(const uint8_t* row, uint32_t b0, uint32_t nb) {
@@ -201,7 +194,7 @@ __device__ __forceinline__ uint32_t top_scale(const uint4& s) {
 // All but the inputs' stages: codes, factors, each drain warp's factors
 // and output places, barriers, and the alignment's slack.
 __host__ __device__ constexpr uint32_t fixed_bytes(int tn) {
-  return kCodes * kRows * 64 + kScaleSlots * kRows * 4 + 8 * (tn / 2) * 12 + 1024 + 1024;
+  return kCodes * kRows * 128 + kScaleSlots * kRows * 4 + 8 * (tn / 2) * 12 + 1024 + 1024;
 }
 __host__ __device__ constexpr uint32_t stages_of(int parts, int tn) {
   return (kSmemBudget - fixed_bytes(tn)) / (uint32_t)(parts * tn * 128) < kMaxStages
@@ -217,16 +210,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     tile_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw, const Args a,
                 long long wait_cycles, int* __restrict__ err) {
   constexpr uint32_t N = PARTS * TN;  // the MMA's columns
-  constexpr uint32_t S = stages_of(PARTS, TN), kCols = 2 * N + 32 * kWide <= 256 ? 256 : 512;
+  constexpr uint32_t S = stages_of(PARTS, TN), kCols = 512;
   // Tensor memory: a run's sums, two where they fit, and the widened weights.
-  constexpr uint32_t kSums = 2 * N + 32 * kWide <= 512 ? 2 : 1;
+  // Each slab of those is 32 columns.
+  constexpr uint32_t kSums = N <= 160 ? 2 : 1, kWide = N == 160 ? 6 : 8;
   static_assert(kSums * N + 32 * kWide <= 512, "tensor memory");
   constexpr uint32_t kHalf = TN / 2;  // a drain warp's tokens
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (an offset, so that the loads stay shared memory's)
   uint8_t* xs = smem;                            // [S][N rows][128 bytes]
-  uint8_t* raw = xs + S * N * 128;               // [kCodes][128 rows][64 bytes]
-  uint64_t* places = reinterpret_cast<uint64_t*>(raw + kCodes * kRows * 64);  // [8 drain warps][kHalf]
+  uint8_t* raw = xs + S * N * 128;               // [kCodes][128 rows][128 bytes]
+  uint64_t* places = reinterpret_cast<uint64_t*>(raw + kCodes * kRows * 128);  // [8 drain warps][kHalf]
   float* swb = reinterpret_cast<float*>(places + 8 * kHalf);         // [kScaleSlots][128]
   float* sxb = swb + kScaleSlots * kRows;                            // [8 drain warps][kHalf]
   uint64_t* bars = reinterpret_cast<uint64_t*>(sxb + 8 * kHalf);
@@ -239,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t slabs = (a.kk + kSlab - 1) / kSlab;
-  const uint32_t pairs = (a.kk + kPairK - 1) / kPairK;  // of slabs, the last perhaps one
+  const uint32_t halves = (a.kk + kHalfK - 1) / kHalfK;
 
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < kDone; ++s) {
@@ -248,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (uint32_t s = 0; s < kCodes; ++s) {
       mbar_init(smem_u32(&rfull[s]), 1);
-      mbar_init(smem_u32(&rempty[s]), 4);
+      mbar_init(smem_u32(&rempty[s]), kWidenWarps);  // all of them wait for every stage: none may miss its turn
     }
     for (uint32_t s = 0; s < 2; ++s) {
       mbar_init(smem_u32(&afull[s]), 1);
@@ -384,14 +378,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp < 8 + kWidenWarps) {
     other_registers<TN>();
-    // Widen: sets of four warps take pairs of slabs in turn, a thread a row
-    // (its TMEM lane): 64 bytes of codes (chunk c of row r at c ^ (r / 2 %
-    // 4), the 64-byte swizzle) to twice 32 columns of binary16 pairs.
-    const uint32_t id = threadIdx.x - 256, row = id & 127, set = id >> 7, turn4 = (row >> 1) & 3;
+    // Widen: a set of four warps takes the first half of every run, the other
+    // the second, a thread a row (its TMEM lane): a slab is 32 bytes of codes
+    // (chunk c of row r's 128 bytes at c ^ (r % 8), the 128-byte swizzle) to
+    // 32 columns of binary16 pairs.
+    const uint32_t id = threadIdx.x - 256, row = id & 127, set = id >> 7, turn = row & 7;
     const uint32_t nb = a.kk / mx::kBlock;
-    const uint8_t* from = raw + row * 64;
+    const uint8_t* from = raw + row * 128;
     const uint32_t to = tmem + ((32 * (warp & 3)) << 16) + kSums * N;
-    uint32_t i = 0, s = 0, q = 0, g = 0;  // slabs so far, their place in the ring, pairs, runs
+    uint32_t i0 = 0, q = 0, g = 0;  // slabs, stages of codes and runs so far
     auto scales_of = [&](const Piece& p) {
       return a.scales + ((size_t)p.e * a.n + min(p.row0 + row, a.n - 1)) * nb;
     };
@@ -423,53 +418,59 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&sfull[g % kScaleSlots]));
         }
-        const uint32_t end = min((run + 1) * (kRun / kPairK), pairs);
+        // This set's eight blocks' scales; and what takes a scale byte to a
+        // binary32 exponent: 2^(byte - ref + 12).
+        const uint32_t mine[2] = {set ? sc.z : sc.x, set ? sc.w : sc.y};
+        const int bias = 139 - ref;
+        const uint32_t left = slabs - run * (kRun / kSlab);  // of the tile
 #pragma unroll 1
-        for (uint32_t d = run * (kRun / kPairK); d < end; ++d, ++q) {
-          const bool two = 2 * d + 1 < slabs;
-          if (q % kSets == set) {
-            const uint32_t rs = q % kCodes, w = d % 4;
-            const uint32_t four = w < 2 ? (w == 0 ? sc.x : sc.y) : (w == 2 ? sc.z : sc.w);  // the blocks' scales
-            if (!(ok = wait(&rfull[rs], (q / kCodes) & 1, LT_TIMEOUT_CODES))) break;
+        for (uint32_t half = 0; half < 2 && 4 * half < left; ++half, ++q) {
+          if (!(ok = wait(&rfull[q % kCodes], (q / kCodes) & 1, LT_TIMEOUT_CODES))) break;
+          if (half != set) {
+            if (lane == 0) mbar_arrive(smem_u32(&rempty[q % kCodes]));
+            continue;
+          }
+          const uint8_t* stage = from + (q % kCodes) * kRows * 128;
 #pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) {
-              if (h == 1 && !two) break;
-              const uint32_t at = to + 32 * (h == 0 ? s : s + 1 == kWide ? 0 : s + 1);
+          for (uint32_t h = 0; h < 4; ++h) {
+            if (4 * half + h >= left) break;
+            const uint32_t i = i0 + 4 * half + h;
+            const uint32_t at = to + 32 * (i % kWide);
 #pragma unroll
-              for (uint32_t c = 0; c < 2; ++c) {
-                const uint4 v = *reinterpret_cast<const uint4*>(from + rs * kRows * 64 + (((2 * h + c) ^ turn4) << 4));
-                const uint32_t byte = (four >> (8 * (2 * h + c))) & 0xFFu;
-                const uint32_t by = byte == 255 ? 0x7E007E00u : half_power2((int)byte - ref + 12);
-                const uint32_t words[4] = {v.x, v.y, v.z, v.w};
-                uint32_t wide[16];
+            for (uint32_t c = 0; c < 2; ++c) {
+              const uint4 v = *reinterpret_cast<const uint4*>(stage + (((2 * h + c) ^ turn) << 4));
+              const uint32_t byte = (mine[h / 2] >> (16 * (h % 2) + 8 * c)) & 0xFFu;
+              // Binary16's own range does the rest: subnormal, then 0.
+              const float power = __uint_as_float((uint32_t)max((int)byte + bias, 0) << 23);
+              uint32_t by;
+              asm("cvt.rn.f16x2.f32 %0, %1, %1;" : "=r"(by) : "f"(byte == 255 ? __uint_as_float(0x7FC00000u) : power));
+              const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+              uint32_t wide[16];
 #pragma unroll
-                for (uint32_t u = 0; u < 4; ++u) {
-                  uint32_t f[4];
-                  mx::widen8_f16(words[u], f);
+              for (uint32_t u = 0; u < 4; ++u) {
+                uint32_t f[4];
+                mx::widen8_f16(words[u], f);
 #pragma unroll
-                  for (int e = 0; e < 4; ++e)
-                    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(wide[4 * u + e]) : "r"(f[e]), "r"(by));
-                }
-                // Half a slab is widened in registers while its columns may still be in use.
-                if (c == 0 && i + h >= kWide) {
-                  const uint32_t before = i + h - kWide;
-                  if (!(ok = wait(done_bar(before), before / kDone & 1, LT_TIMEOUT_MMA))) break;
-                }
-                tmem_st16(at + 16 * c, wide);
+                for (int e = 0; e < 4; ++e)
+                  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(wide[4 * u + e]) : "r"(f[e]), "r"(by));
               }
-              if (!ok) break;
-              tmem_wait_st();
-              fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(smem_u32(&full[(i + h) % kDone]));
+              // Half a slab is widened in registers while its columns may still be in use.
+              if (c == 0 && i >= kWide) {
+                const uint32_t before = i - kWide;
+                if (!(ok = wait(done_bar(before), before / kDone & 1, LT_TIMEOUT_MMA))) break;
+              }
+              tmem_st16(at + 16 * c, wide);
             }
             if (!ok) break;
-            if (lane == 0) mbar_arrive(smem_u32(&rempty[rs]));
+            tmem_wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&full[i % kDone]));
           }
-          i += two ? 2 : 1;
-          s += two ? 2 : 1;
-          if (s >= kWide) s -= kWide;
+          if (!ok) break;
+          if (lane == 0) mbar_arrive(smem_u32(&rempty[q % kCodes]));
         }
+        i0 += min(left, kRun / kSlab);
       }
     }
   } else {
@@ -492,16 +493,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     // (or, where a wait ran out, their bytes have come, within limits).
     for (uint32_t j = i > S ? i - S : 0; j < i; ++j) wait1(&full[j % kDone], j / kDone & 1, LT_TIMEOUT_INPUTS);
   } else if (warp == kCodeWarp && elect_one()) {
-    // Codes: a pair of slabs a stage.
+    // Codes: half a run a stage.
     uint32_t q = 0;
     bool ok = true;
     while (ok && work.next(a, o))
-      for (uint32_t r = o.r0 * (kRun / kPairK), end = min(o.r1 * (kRun / kPairK), pairs); r < end; ++r, ++q) {
+      for (uint32_t r = o.r0 * (kRun / kHalfK), end = min(o.r1 * (kRun / kHalfK), halves); r < end; ++r, ++q) {
         const uint32_t s = q % kCodes;
         if (q >= kCodes && !(ok = wait1(&rempty[s], (q / kCodes - 1) & 1, LT_TIMEOUT_WIDEN))) break;
         const uint32_t bar = smem_u32(&rfull[s]);
-        mbar_expect_tx(bar, kRows * 64);
-        tma_load_3d(smem_u32(raw + s * kRows * 64), &tw, (int)(r * 64), (int)o.row0, (int)o.e, bar);
+        mbar_expect_tx(bar, kRows * 128);
+        tma_load_3d(smem_u32(raw + s * kRows * 128), &tw, (int)(r * 128), (int)o.row0, (int)o.e, bar);
       }
     for (uint32_t j = q > kCodes ? q - kCodes : 0; j < q; ++j)
       wait1(&rfull[j % kCodes], (j / kCodes) & 1, LT_TIMEOUT_CODES);
@@ -718,10 +719,10 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn_lt() {
   return fn;
 }
 
-// [depth][rows][width] elements as boxes of box_w x box_rows x 1, swizzled
-// over 128 or 64 bytes; what lies past any of the three reads as zeros.
+// [depth][rows][width] elements as boxes of box_w x box_rows x 1, 128-byte
+// swizzle; what lies past any of the three reads as zeros.
 bool make_map_lt(CUtensorMap* map, CUtensorMapDataType type, uint32_t elem, const void* base, uint64_t width,
-                 uint64_t rows, uint64_t depth, uint32_t box_w, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+                 uint64_t rows, uint64_t depth, uint32_t box_w, uint32_t box_rows) {
   auto fn = encode_fn_lt();
   if (!fn) return false;
   cuuint64_t dims[3] = {width, rows, depth};
@@ -729,7 +730,7 @@ bool make_map_lt(CUtensorMap* map, CUtensorMapDataType type, uint32_t elem, cons
   cuuint32_t box[3] = {box_w, box_rows, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   return fn(map, type, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -739,10 +740,8 @@ cudaError_t launch_tile(const FkLinearMx& a, const fk::lt::Args& g, const uint16
   using namespace fk::lt;
   constexpr size_t smem = smem_of(PARTS, TN);
   CUtensorMap tx, tw;
-  if (!make_map_lt(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, parts, a.kk, g.slots, PARTS, kSlab, TN,
-                   CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !make_map_lt(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.kk / 2, a.n, a.entries, kPairK / 2, kRows,
-                   CU_TENSOR_MAP_SWIZZLE_64B))
+  if (!make_map_lt(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, parts, a.kk, g.slots, PARTS, kSlab, TN) ||
+      !make_map_lt(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.kk / 2, a.n, a.entries, kHalfK / 2, kRows))
     return cudaErrorInvalidValue;
   cudaError_t e = fk_allow_smem(tile_kernel<E, PARTS, TN>, smem < 120 * 1024 ? 120 * 1024 : smem);
   if (e != cudaSuccess) return e;
@@ -774,17 +773,27 @@ cudaError_t launch_all(const FkLinearMx& a, int sms, int* err, bool pdl, cudaStr
     perm = reinterpret_cast<uint32_t*>(take(4 * pairs));
     slot_of = reinterpret_cast<uint32_t*>(take(4 * pairs));
   }
-  // The token tile that costs an expert's mean share least: a slab of a tile
-  // of N = PARTS tn columns takes the MMAs 2 N cycles, and the widening warps
-  // about 250 whatever N is.
-  const uint64_t share = (pairs + a.entries - 1) / a.entries;
+  // The token tile that costs least. In units of 2.2 ns: the slabs of an
+  // SM's tiles, whose costs by width are measured (22016 x 4096 by 511 rows:
+  // f32 in tiles of 16, 32, 64 and 128 tokens 531, 281, 184 and 160 us; bf16
+  // of 16, 32, 64 and 160 528, 274, 151 and 100), and the last tiles' sums,
+  // which nothing covers (11008 x 4096 by 128 f32 rows: 64 tokens 31 us, 128
+  // 38; by 64 rows 24 and 45). Routed experts are uneven: half a tile of
+  // each is taken to be empty (64 experts with 32 pairs on average, 2816 x
+  // 2048: 32 tokens 134 us, 64 118, 128 181).
+  constexpr uint32_t kWidths = 4;
+  const uint32_t widths[kWidths] = {16, 32, 64, PARTS == 2 ? 128 : 160};
+  const double slab_cost[kWidths] = {100, PARTS == 2 ? 106 : 104, PARTS == 2 ? 139 : 114, PARTS == 2 ? 240 : 151};
+  const uint32_t wtiles = (a.n + kRows - 1) / kRows;
+  const double used = pairs < a.entries ? (double)pairs : (double)a.entries;
+  const double slabs = used * wtiles * ((a.kk + kSlab - 1) / kSlab) / sms;
   uint32_t tn = 16;
-  uint64_t least = ~0ull;
-  constexpr uint32_t kWidest = PARTS == 2 ? 128 : 160;
-  const uint32_t widths[] = {16, 32, 64, 160 / PARTS, kWidest};
-  for (uint32_t w : widths) {
-    const uint64_t slab = 2 * PARTS * w > 250 ? 2 * PARTS * w : 250, cost = (share + w - 1) / w * (slab + w / 4);
-    if (cost < least) least = cost, tn = w;
+  double least = 0;
+  for (uint32_t i = 0; i < kWidths; ++i) {
+    const double share = (double)pairs / used / widths[i];
+    const double tiles = !a.ids ? (double)((pairs + widths[i] - 1) / widths[i]) : share > 0.5 ? share + 0.5 : 1.0;
+    const double cost = tiles * slabs * slab_cost[i] + 70.0 * widths[i];
+    if (i == 0 || cost < least) least = cost, tn = widths[i];
   }
   if (a.ids) {
     cudaError_t e = fk_launch_ex(group_kernel, dim3(1), dim3(1024), 0, s, pdl, a.ids, (uint32_t)pairs, a.entries, tn,
@@ -793,7 +802,6 @@ cudaError_t launch_all(const FkLinearMx& a, int sms, int* err, bool pdl, cudaStr
   }
   // A CTA an SM, each an equal share of the tiles' runs, where the parts of
   // tiles that they leave find room in the workspace; else of whole tiles.
-  const uint32_t wtiles = (a.n + kRows - 1) / kRows;
   const uint64_t most =
       (a.ids ? pairs / tn + (pairs < a.entries ? pairs : (uint64_t)a.entries) : (pairs + tn - 1) / tn) * wtiles;  // tiles at most
   uint64_t grid = most < (uint64_t)sms ? most : (uint64_t)sms;
@@ -819,8 +827,7 @@ cudaError_t launch_all(const FkLinearMx& a, int sms, int* err, bool pdl, cudaStr
     case 16: return launch_tile<E, PARTS, 16>(a, g, parts, ctas, err, pdl, s);
     case 32: return launch_tile<E, PARTS, 32>(a, g, parts, ctas, err, pdl, s);
     case 64: return launch_tile<E, PARTS, 64>(a, g, parts, ctas, err, pdl, s);
-    case 160 / PARTS: return launch_tile<E, PARTS, 160 / PARTS>(a, g, parts, ctas, err, pdl, s);
-    default: return launch_tile<E, PARTS, kWidest>(a, g, parts, ctas, err, pdl, s);
+    default: return launch_tile<E, PARTS, PARTS == 2 ? 128 : 160>(a, g, parts, ctas, err, pdl, s);
   }
 }
 

@@ -305,6 +305,21 @@ def test_routed_uneven(ctx, m):
         held_to_experts(y, codes, scales, ids, x, "f32", False)
 
 
+@pytest.mark.parametrize("entries,n,kk,m,k", [(16, 1300, 2080, 400, 8), (16, 2600, 4096, 600, 8)])
+@pytest.mark.parametrize("t", TYPES)
+def test_routed_many_tiles(ctx, entries, n, kk, m, k, t):
+    """Several tiles a block, several runs a tile, uneven experts, one without
+    rows; held at some of the columns."""
+    codes = O.ints(381, entries * n * kk // 2, 256).astype(np.uint8).reshape(entries, n, kk // 2)
+    scales = (120 + O.ints(382, entries * n * kk // 32, 5)).astype(np.uint8).reshape(entries, n, kk // 32)
+    ids = np.minimum(O.ints(383, m * k, entries), O.ints(384, m * k, entries)).reshape(m, k)
+    ids[ids == 2] = 9
+    x = O.normal(385, m * kk).reshape(m, kk)
+    y = routed(ctx, codes, scales, ids, x, t, False)
+    at = np.unique(np.concatenate([[0, 127, 128, n - 1], O.ints(386, 24, n)]))
+    held_to_experts(y[:, :, at], codes[:, at], scales[:, at], ids, x, t, False)
+
+
 @pytest.mark.parametrize("m", [4, 120])
 def test_routed_same_every_time(ctx, m):
     entries, n, kk, k = 8, 256, 1024, 4
