@@ -35,31 +35,34 @@ constexpr uint32_t kStageBlocks = 8;   // blocks of 32 weights a row a stage: 12
 constexpr uint32_t kCodeBytes = kTileRows * kStageBlocks * 16;
 constexpr uint32_t kScaleWords = 3;    // the words that hold 8 bytes, wherever they start
 constexpr uint32_t kMaxPairs = 512;
+constexpr uint32_t kBatch = 8, kLeastBatch = 4;  // units whose sums wait together: at best, where shared memory is short
 constexpr uint32_t kMaxEntries = 4096;
 constexpr uint32_t kSmemBudget = 227 * 1024 - 1024;  // static and dynamic, less the alignment's slack
 
 enum { LS_TIMEOUT = 29 };  // a stage of codes never landed
 
 // Stages of a warp's own ring.
-__host__ __device__ constexpr uint32_t stages_of(uint32_t R) { return R <= 4 ? 3 : 2; }
+constexpr uint32_t kStages = 3;
 
 // A stage's scale words and their values as factors.
 constexpr uint32_t kScaleBytes = kTileRows * kScaleWords * 4;
 constexpr uint32_t kFactorBytes = kTileRows * kStageBlocks * 4;
 
-// A warp's inputs: `steps` stages of R rows, two parts of 512 bytes each,
+// A group's inputs: `steps` stages of R rows, two parts of 512 bytes each,
 // and a factor a row and stage.
 __host__ __device__ constexpr uint32_t input_bytes(uint32_t steps, uint32_t R) {
   return steps * R * kStageBlocks * 128 + (steps * R * 4 + 15) / 16 * 16;
 }
-__host__ __device__ constexpr uint32_t warp_bytes(uint32_t steps, uint32_t R) {
-  return stages_of(R) * (kCodeBytes + kScaleBytes) + kFactorBytes + input_bytes(steps, R);
+// A warp's scale words and factors, and all of a block's shared memory.
+constexpr uint32_t kOwnBytes = kStages * kScaleBytes + kFactorBytes;
+// Units whose sums wait together: `batch` of them.
+__host__ __device__ constexpr uint32_t sum_bytes(uint32_t batch, uint32_t R) {
+  return batch * kWarps * kTileRows * R * 4;
 }
-// Units whose sums wait together.
-__host__ __device__ constexpr uint32_t batch_of(uint32_t R) { return R <= 4 ? 8 : 4; }
-__host__ __device__ constexpr uint32_t static_bytes(uint32_t R) {
-  return kMaxPairs * 12 + kThreads * 4 + batch_of(R) * kWarps * kTileRows * R * 4 + 1024 + kWarps * stages_of(R) * 8;
+__host__ __device__ constexpr uint32_t block_bytes(uint32_t steps, uint32_t share, uint32_t batch, uint32_t R) {
+  return kWarps * (kStages * kCodeBytes + kOwnBytes) + kWarps / share * input_bytes(steps, R) + sum_bytes(batch, R);
 }
+constexpr uint32_t kStaticBytes = kMaxPairs * 12 + kThreads * 4 + 1024 + kWarps * kStages * 8;
 
 // Four bytes, of which `have` are there (the others become 0).
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src, uint32_t have) {
@@ -92,21 +95,19 @@ struct Pass {
 // others.
 template <class E, int R>
 __global__ void __launch_bounds__(kThreads, 1)
-    stream_kernel(const __grid_constant__ CUtensorMap tw, const FkLinearMx a, uint32_t share,
+    stream_kernel(const __grid_constant__ CUtensorMap tw, const FkLinearMx a, uint32_t share, uint32_t batch,
                   long long wait_cycles, int* __restrict__ err) {
-  constexpr int NT = (R + 3) / 4;  // products of 8 columns
-  constexpr uint32_t kBatch = batch_of(R), stages = stages_of(R);
+  constexpr uint32_t stages = kStages;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t landed[kWarps][stages];
   __shared__ Pass passes[kMaxPairs];
   __shared__ uint32_t perm[kMaxPairs];  // a pair's row, its rank << 16
   __shared__ uint32_t ids_s[kThreads];
-  __shared__ float red[kBatch][kWarps][kTileRows * R];
   __shared__ uint32_t sums[2][kWarps], npasses_s, nrest_s;
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (an offset, so that the loads stay shared memory's)
   const uint32_t blocks = a.kk / mx::kBlock, all_steps = (blocks + kStageBlocks - 1) / kStageBlocks;
-  const uint32_t most_steps = (all_steps + share - 1) / share;
-  // [kWarps][stages] codes, then a warp's scale words, factors and inputs.
+  // [kWarps][stages] codes, each warp's scale words and factors, each group's inputs,
+  // [batch][kWarps][R][16] sums.
   uint8_t* rest_smem = smem + kWarps * stages * kCodeBytes;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const uint32_t pairs = a.m * a.k, tiles = (a.n + kTileRows - 1) / kTileRows;
@@ -192,13 +193,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t s0 = part * all_steps / share, steps = (part + 1) * all_steps / share - s0;
   const uint64_t scale_bytes = (uint64_t)a.entries * a.n * blocks;
   const uint32_t ring = smem_u32(smem) + warp * stages * kCodeBytes;
-  uint8_t* mine_smem = rest_smem + warp * (warp_bytes(most_steps, R) - stages * kCodeBytes);
+  uint8_t* mine_smem = rest_smem + warp * kOwnBytes;
   const uint32_t scale_ring = smem_u32(mine_smem);
   float* factors = reinterpret_cast<float*>(mine_smem + stages * kScaleBytes);  // [16 rows][8]
   // The inputs, [blocks][R][4][2] 16 bytes as the products take them, and
-  // the factors back, [steps][R].
-  uint8_t* xs = reinterpret_cast<uint8_t*>(factors) + kFactorBytes;
-  float* sxs = reinterpret_cast<float*>(xs + most_steps * kStageBlocks * R * 128);
+  // the factors back, [steps][R]: this warp's of its group's.
+  uint8_t* group_smem = rest_smem + kWarps * kOwnBytes + group * input_bytes(all_steps, R);
+  auto red = reinterpret_cast<float(*)[kWarps][kTileRows * R]>(rest_smem + kWarps * kOwnBytes +
+                                                               abreast * input_bytes(all_steps, R));
+  uint8_t* xs = group_smem + s0 * kStageBlocks * R * 128;
+  float* sxs = reinterpret_cast<float*>(group_smem + all_steps * kStageBlocks * R * 128) + s0 * R;
 
   // A unit's first row, and where this warp's scale bytes of row `of` of it
   // start. A unit's rows end with the table's: the last unit starts early
@@ -302,9 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // Where the scale bytes of row lane / 2 lie in their words (a stage moves on by whole words).
     if (tile == 0 || tile + 1 == tiles || u == u0) shift = 8 * ((uint32_t)first_scale(pass, tile, lane >> 1) & 3u);
-    float acc[NT][2];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = 0.0f;
+    float acc0 = 0.0f, acc1 = 0.0f;
     // Columns without a row take another's (R < 4) or what is there: each
     // column is its own, and theirs are not stored.
     const uint4* xat = reinterpret_cast<const uint4*>(xs) + (((g >> 1) % R) * 4 + t) * 2 + (g & 1);
@@ -341,9 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       const uint8_t* st = smem + (warp * stages + slot) * kCodeBytes + g * 128 + t * 4;
       const float4* fg = reinterpret_cast<const float4*>(factors) + 2 * g;
-      float sum[NT][2];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) sum[j][0] = sum[j][1] = 0.0f;
+      float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
       for (uint32_t b4 = 0; b4 < kStageBlocks; b4 += 4) {
         const float4 f0 = fg[b4 / 4], f1 = fg[16 + b4 / 4];
@@ -356,38 +356,30 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t p[4], q[4];
           mx::widen8_f16(*reinterpret_cast<const uint32_t*>(at), p);
           mx::widen8_f16(*reinterpret_cast<const uint32_t*>(at + 8 * 128), q);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            const uint4 x = xat[(b * R + 4 * j) * 8];
-            float d[4];
-            mma0(d, p[0], q[0], p[1], q[1], x.x, x.y);
-            mma(d, p[2], q[2], p[3], q[3], x.z, x.w);
-            sum[j][0] = fmaf(__fadd_rn(d[0], d[1]), s0v[bb], sum[j][0]);
-            sum[j][1] = fmaf(__fadd_rn(d[2], d[3]), s1v[bb], sum[j][1]);
-          }
+          const uint4 x = xat[b * R * 8];
+          float d[4];
+          mma0(d, p[0], q[0], p[1], q[1], x.x, x.y);
+          mma(d, p[2], q[2], p[3], q[3], x.z, x.w);
+          sum0 = fmaf(__fadd_rn(d[0], d[1]), s0v[bb], sum0);
+          sum1 = fmaf(__fadd_rn(d[2], d[3]), s1v[bb], sum1);
         }
       }
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const float sx = sat[4 * j];
-        acc[j][0] = fmaf(sum[j][0], sx, acc[j][0]);
-        acc[j][1] = fmaf(sum[j][1], sx, acc[j][1]);
-      }
+      const float sx = *sat;
+      acc0 = fmaf(sum0, sx, acc0);
+      acc1 = fmaf(sum1, sx, acc1);
       xat += kStageBlocks * R * 8, sat += R;
       if (++slot == stages) slot = 0, phase ^= 1;
       __syncwarp();  // before the stage is loaded again
     }
-    // The warps' sums of up to kBatch units are added together at once: a
+    // The warps' sums of up to `batch` units are added together at once: a
     // barrier a unit, and the adding behind it, held the warps up for as
     // long as half a unit's products.
     float(*rd)[kTileRows * R] = red[held];
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-      if (4 * j + t < (uint32_t)R) {
-        rd[warp][(4 * j + t) * kTileRows + g] = acc[j][0];
-        rd[warp][(4 * j + t) * kTileRows + g + 8] = acc[j][1];
-      }
-    if (++held < kBatch && u + 1 < u1) continue;
+    if (t < (uint32_t)R) {
+      rd[warp][t * kTileRows + g] = acc0;
+      rd[warp][t * kTileRows + g + 8] = acc1;
+    }
+    if (++held < batch && u + 1 < u1) continue;
     group_sync();
     for (uint32_t o = part * 32 + lane; o < held * (kTileRows * R); o += 32 * share) {
       const uint32_t uo = u + 1 - held + o / (kTileRows * R), i = o % (kTileRows * R);
@@ -414,7 +406,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // How many warps share a unit: the fewest rounds of units, each its blocks
-// a warp and about 8 blocks' worth of fixed cost, whose inputs fit. 0: none.
+// a warp and about 8 blocks' worth of fixed cost, and the inputs' splitting
+// before them, whose inputs fit (4096 x 11008 by one row: 16 warps 11.4 us, 8
+// 12.9). 0: none.
 inline uint32_t share_of(uint64_t units, uint32_t blocks, uint32_t R, int sms) {
   uint32_t best = 0;
   uint64_t least = ~0ull;
@@ -422,8 +416,8 @@ inline uint32_t share_of(uint64_t units, uint32_t blocks, uint32_t R, int sms) {
   for (uint32_t share = kWarps; share >= 1; share /= 2) {
     const uint32_t steps = (all + share - 1) / share;
     const uint64_t at_once = (uint64_t)sms * (kWarps / share);
-    const uint64_t cost = (units + at_once - 1) / at_once * (steps * kStageBlocks + 8);
-    if (static_bytes(R) + (uint64_t)kWarps * warp_bytes(steps, R) <= kSmemBudget && cost < least)
+    const uint64_t cost = (units + at_once - 1) / at_once * (steps * kStageBlocks + 8) + 4 * steps;
+    if (kStaticBytes + block_bytes(all, share, kLeastBatch, R) <= kSmemBudget && cost < least)
       least = cost, best = share;
   }
   return best;
@@ -453,16 +447,17 @@ template <class E, int R>
 cudaError_t launch(const FkLinearMx& a, uint32_t share, int sms, int* err, bool pdl, cudaStream_t s) {
   const uint64_t pairs = (uint64_t)a.m * a.k, tiles = (a.n + kTileRows - 1) / kTileRows;
   const uint32_t all = (a.kk / mx::kBlock + kStageBlocks - 1) / kStageBlocks;
-  size_t rest = (size_t)kWarps * (warp_bytes((all + share - 1) / share, R) - stages_of(R) * kCodeBytes);
+  const uint32_t batch = kStaticBytes + block_bytes(all, share, kBatch, R) <= kSmemBudget ? kBatch : kLeastBatch;
+  size_t rest = block_bytes(all, share, batch, R) - (size_t)kWarps * kStages * kCodeBytes;
   if (a.ids && rest < (a.entries + kThreads) * 4) rest = (a.entries + kThreads) * 4;  // the count's space
-  const size_t smem = 1024 + (size_t)kWarps * stages_of(R) * kCodeBytes + rest;
+  const size_t smem = 1024 + (size_t)kWarps * kStages * kCodeBytes + rest;
   CUtensorMap tw;
   if (!code_map(&tw, a)) return cudaErrorInvalidValue;
   cudaError_t e = fk_allow_smem(stream_kernel<E, R>, smem);
   if (e != cudaSuccess) return e;
   const uint64_t most = (pairs * tiles + kWarps / share - 1) / (kWarps / share);  // blocks that have a unit
   return fk_launch_ex(stream_kernel<E, R>, dim3((uint32_t)(most < (uint64_t)sms ? most : (uint64_t)sms)),
-                      dim3(kThreads), smem, s, pdl, tw, a, share, (long long)4000000000LL, err);
+                      dim3(kThreads), smem, s, pdl, tw, a, share, batch, (long long)4000000000LL, err);
 }
 
 }  // namespace ls
@@ -473,18 +468,26 @@ size_t fk_linear_mxfp4_work(uint64_t entries, uint64_t n, uint64_t kk, uint64_t 
   return 5 * pairs * kk + 16 * (pairs < 512 ? pairs : 512) * n + 16 * pairs + 64 * entries + 65536;
 }
 
+// Weights that are read twice rather than widened by the tile kernel, whose
+// launches and first loads cost more than a second pass over few of them (8
+// rows by 4096 x 4096: 11.1 us in two passes, 20.0 in tiles; 11008 x 4096:
+// 19.3 and 22.5; 32000 x 4096: 42.8 and 32.4).
+constexpr uint64_t kTwice = 64u << 20;
+
 cudaError_t fk_launch_linear_mxfp4(const FkLinearMx& a, FkElem e, int sms, int* err, bool pdl, cudaStream_t s) {
   if (a.m == 0 || a.n == 0) return cudaSuccess;
   if (a.kk == 0 || a.kk % fk::mx::kBlock != 0 || a.k == 0 || a.entries == 0 || a.entries > fk::ls::kMaxEntries ||
       a.ldx < (uint64_t)a.kk * (a.per_rank ? a.k : 1) || a.ldy < (uint64_t)a.k * a.n)
     return cudaErrorInvalidValue;
   const uint64_t pairs = (uint64_t)a.m * a.k;
-  if (pairs <= fk::ls::kMaxPairs && pairs <= 8ull * a.entries && a.n >= fk::ls::kTileRows) {
-    // Rows a pass: 4 where an expert has that many on average, 8 past it,
-    // fewer where there are no more or where they do not fit.
-    uint32_t R = pairs <= 2 ? (uint32_t)pairs : pairs <= 4ull * a.entries ? 4 : 8;
+  const uint64_t experts = a.ids && pairs > a.entries ? a.entries : a.ids ? pairs : 1;  // at most
+  // Up to 4 pairs an expert on average, a pass over its weights; up to 8,
+  // two, where the weights are few.
+  if (pairs <= fk::ls::kMaxPairs && a.n >= fk::ls::kTileRows &&
+      (pairs <= 4ull * a.entries || (pairs <= 8ull * a.entries && experts * a.n * a.kk <= kTwice))) {
+    // Rows a pass: 4, fewer where there are no more or where they do not fit.
+    uint32_t R = pairs <= 2 ? (uint32_t)pairs : 4;
     uint32_t share = 0;
-    const uint64_t experts = a.ids && pairs > a.entries ? a.entries : a.ids ? pairs : 1;  // at most
     for (; R >= 1; R /= 2) {
       const uint64_t passes = a.ids ? experts : (pairs + R - 1) / R;
       share = fk::ls::share_of(passes * ((a.n + fk::ls::kTileRows - 1) / fk::ls::kTileRows), a.kk / 32, R, sms);
@@ -493,8 +496,7 @@ cudaError_t fk_launch_linear_mxfp4(const FkLinearMx& a, FkElem e, int sms, int* 
 #define FK_CALL(E)                                              \
   (R == 1   ? fk::ls::launch<E, 1>(a, share, sms, err, pdl, s)   \
    : R == 2 ? fk::ls::launch<E, 2>(a, share, sms, err, pdl, s)   \
-   : R == 4 ? fk::ls::launch<E, 4>(a, share, sms, err, pdl, s)   \
-            : fk::ls::launch<E, 8>(a, share, sms, err, pdl, s))
+            : fk::ls::launch<E, 4>(a, share, sms, err, pdl, s))
     if (share) return FK_BY_ELEM(e, FK_CALL);
 #undef FK_CALL
   }

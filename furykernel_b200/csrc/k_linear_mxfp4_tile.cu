@@ -63,9 +63,9 @@ __device__ __forceinline__ void other_registers() {
   else
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
 }
-constexpr uint32_t kMaxStages = 16;   // of inputs: a load takes 1000 to 3000 cycles to land
+constexpr uint32_t kMaxSlabs = 16;    // of inputs held: a load takes 1000 to 3000 cycles to land
 constexpr uint32_t kCodes = 4;        // stages of codes
-constexpr uint32_t kDone = 32;        // slabs whose MMAs' end is told apart
+constexpr uint32_t kDone = 32;        // steps whose MMAs' end is told apart
 constexpr uint32_t kScaleSlots = 12;  // runs whose factors are held
 constexpr uint32_t kSmemBudget = 226 * 1024;
 constexpr uint32_t kMaxEntries = 4096;
@@ -191,18 +191,26 @@ __device__ __forceinline__ uint32_t top_scale(const uint4& s) {
   return m;
 }
 
+// Slabs a step, of tiles of n columns. A step is what one set of barriers
+// stands for: the MMA warp's round of waits and commit takes about 200 cycles
+// beside its MMAs, which up to 128 columns take 40 to 64 each, so that two
+// slabs share a round there (32000 x 4096 by 32 bf16 rows 35.0 -> 33.2 us, 64
+// experts of 2816 x 2048 by 511 x 4 f32 pairs 116 -> 107).
+__host__ __device__ constexpr uint32_t step_of(int n) { return n <= 128 ? 2 : 1; }
 // All but the inputs' stages: codes, factors, each drain warp's factors
 // and output places, barriers, and the alignment's slack.
-__host__ __device__ constexpr uint32_t fixed_bytes(int tn) {
+__host__ __device__ constexpr uint32_t fixed_bytes(int parts, int tn) {
   return kCodes * kRows * 128 + kScaleSlots * kRows * 4 + 8 * (tn / 2) * 12 + 1024 + 1024;
 }
+__host__ __device__ constexpr uint32_t step_bytes(int parts, int tn) {
+  return step_of(parts * tn) * (uint32_t)(parts * tn * 128);
+}
 __host__ __device__ constexpr uint32_t stages_of(int parts, int tn) {
-  return (kSmemBudget - fixed_bytes(tn)) / (uint32_t)(parts * tn * 128) < kMaxStages
-             ? (kSmemBudget - fixed_bytes(tn)) / (uint32_t)(parts * tn * 128)
-             : kMaxStages;
+  const uint32_t fit = (kSmemBudget - fixed_bytes(parts, tn)) / step_bytes(parts, tn);
+  return fit < kMaxSlabs / step_of(parts * tn) ? fit : kMaxSlabs / step_of(parts * tn);
 }
 __host__ __device__ constexpr uint32_t smem_of(int parts, int tn) {
-  return fixed_bytes(tn) + stages_of(parts, tn) * (uint32_t)(parts * tn * 128);
+  return fixed_bytes(parts, tn) + stages_of(parts, tn) * step_bytes(parts, tn);
 }
 
 template <class E, int PARTS, int TN>
@@ -210,21 +218,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     tile_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw, const Args a,
                 long long wait_cycles, int* __restrict__ err) {
   constexpr uint32_t N = PARTS * TN;  // the MMA's columns
-  constexpr uint32_t S = stages_of(PARTS, TN), kCols = 512;
+  constexpr uint32_t P = step_of(N), S = stages_of(PARTS, TN), kCols = 512;
+  static_assert(S >= 2, "stages of inputs");
   // Tensor memory: a run's sums, two where they fit, and the widened weights.
-  // Each slab of those is 32 columns.
-  constexpr uint32_t kSums = N <= 160 ? 2 : 1, kWide = N == 160 ? 6 : 8;
-  static_assert(kSums * N + 32 * kWide <= 512, "tensor memory");
+  // Each slab of those is 32 columns, each step P slabs.
+  constexpr uint32_t kSums = N <= 160 ? 2 : 1, kWide = (N == 160 ? 6 : 8) / P;
+  static_assert(kSums * N + 32 * P * kWide <= 512, "tensor memory");
   constexpr uint32_t kHalf = TN / 2;  // a drain warp's tokens
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (an offset, so that the loads stay shared memory's)
-  uint8_t* xs = smem;                            // [S][N rows][128 bytes]
-  uint8_t* raw = xs + S * N * 128;               // [kCodes][128 rows][128 bytes]
+  uint8_t* xs = smem;                            // [S][P][N rows][128 bytes]
+  uint8_t* raw = xs + S * P * N * 128;               // [kCodes][128 rows][128 bytes]
   uint64_t* places = reinterpret_cast<uint64_t*>(raw + kCodes * kRows * 128);  // [8 drain warps][kHalf]
   float* swb = reinterpret_cast<float*>(places + 8 * kHalf);         // [kScaleSlots][128]
   float* sxb = swb + kScaleSlots * kRows;                            // [8 drain warps][kHalf]
   uint64_t* bars = reinterpret_cast<uint64_t*>(sxb + 8 * kHalf);
-  // full: a slab's inputs and widened weights; done: its MMAs; rfull and
+  // full: a step's inputs and widened weights; done: its MMAs; rfull and
   // rempty: a stage of codes; afull and aempty: a run's sums; sfull: a run's
   // factors.
   uint64_t *full = bars, *done = full + kDone, *rfull = done + kDone, *rempty = rfull + kCodes,
@@ -282,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     record(err, code);
     return false;
   };
-  // Slab j's MMAs have finished.
+  // Step j's MMAs have finished.
   auto done_bar = [&](uint32_t j) { return &done[j % kDone]; };
 
   if (warp < 8) {
@@ -386,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t nb = a.kk / mx::kBlock;
     const uint8_t* from = raw + row * 128;
     const uint32_t to = tmem + ((32 * (warp & 3)) << 16) + kSums * N;
-    uint32_t i0 = 0, q = 0, g = 0;  // slabs, stages of codes and runs so far
+    uint32_t i0 = 0, q = 0, g = 0;  // steps, stages of codes and runs so far
     auto scales_of = [&](const Piece& p) {
       return a.scales + ((size_t)p.e * a.n + min(p.row0 + row, a.n - 1)) * nb;
     };
@@ -431,11 +440,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             continue;
           }
           const uint8_t* stage = from + (q % kCodes) * kRows * 128;
+          // A step's stores are waited for once a part of the next is widened.
+          auto stored = [&](uint32_t i) {
+            __syncwarp();
+            tmem_wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&full[i % kDone]));
+          };
+          const uint32_t count = min(left - 4 * half, 4u), first = i0 + 4 / P * half;
 #pragma unroll
           for (uint32_t h = 0; h < 4; ++h) {
-            if (4 * half + h >= left) break;
-            const uint32_t i = i0 + 4 * half + h;
-            const uint32_t at = to + 32 * (i % kWide);
+            if (h >= count) break;
+            const uint32_t i = first + h / P, at = to + 32 * (i % kWide * P + h % P);
 #pragma unroll
             for (uint32_t c = 0; c < 2; ++c) {
               const uint4 v = *reinterpret_cast<const uint4*>(stage + (((2 * h + c) ^ turn) << 4));
@@ -454,42 +471,44 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int e = 0; e < 4; ++e)
                   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(wide[4 * u + e]) : "r"(f[e]), "r"(by));
               }
-              // Half a slab is widened in registers while its columns may still be in use.
-              if (c == 0 && i >= kWide) {
-                const uint32_t before = i - kWide;
-                if (!(ok = wait(done_bar(before), before / kDone & 1, LT_TIMEOUT_MMA))) break;
+              // Half a slab is widened in registers while the last step's
+              // stores are on their way and its columns may be in use.
+              if (c == 0 && h % P == 0) {
+                if (h > 0) stored(i - 1);
+                if (i >= kWide && !(ok = wait(done_bar(i - kWide), (i - kWide) / kDone & 1, LT_TIMEOUT_MMA))) break;
+                fence_after();
               }
+              __syncwarp();
               tmem_st16(at + 16 * c, wide);
             }
             if (!ok) break;
-            tmem_wait_st();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&full[i % kDone]));
           }
+          if (ok) stored(first + (count - 1) / P);
           if (!ok) break;
           if (lane == 0) mbar_arrive(smem_u32(&rempty[q % kCodes]));
         }
-        i0 += min(left, kRun / kSlab);
+        i0 += (min(left, kRun / kSlab) + P - 1) / P;
       }
     }
   } else {
   other_registers<TN>();
   if (warp == kInputWarp && elect_one()) {
-    // Inputs: a slab's N rows, the parts one below the other.
+    // Inputs: a step's slabs of N rows, the parts one below the other.
     uint32_t i = 0, s = 0;
     bool ok = true;
     while (ok && work.next(a, o))
-      for (uint32_t slab = o.r0 * (kRun / kSlab), end = min(o.r1 * (kRun / kSlab), slabs); slab < end; ++slab, ++i) {
+      for (uint32_t slab = o.r0 * (kRun / kSlab), end = min(o.r1 * (kRun / kSlab), slabs); slab < end; slab += P, ++i) {
         if (i >= S && !(ok = wait1(done_bar(i - S), (i - S) / kDone & 1, LT_TIMEOUT_MMA))) break;
-        const uint32_t bar = smem_u32(&full[i % kDone]);
-        mbar_expect_tx(bar, N * 128);
+        const uint32_t bar = smem_u32(&full[i % kDone]), count = min(end - slab, P);
+        mbar_expect_tx(bar, count * N * 128);
+        for (uint32_t h = 0; h < count; ++h)
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p)
-          tma_load_3d(smem_u32(xs + s * N * 128 + p * TN * 128), &tx, (int)(slab * kSlab), (int)o.slot0, p, bar);
+          for (int p = 0; p < PARTS; ++p)
+            tma_load_3d(smem_u32(xs + (s * P + h) * N * 128 + p * TN * 128), &tx, (int)((slab + h) * kSlab),
+                        (int)o.slot0, p, bar);
         s = s + 1 == S ? 0 : s + 1;
       }
-    // Loads in flight land before the CTA leaves: the last slabs are done
+    // Loads in flight land before the CTA leaves: the last steps are done
     // (or, where a wait ran out, their bytes have come, within limits).
     for (uint32_t j = i > S ? i - S : 0; j < i; ++j) wait1(&full[j % kDone], j / kDone & 1, LT_TIMEOUT_INPUTS);
   } else if (warp == kCodeWarp && elect_one()) {
@@ -516,15 +535,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (g >= kSums && !(ok = wait1(&aempty[g % kSums], (g / kSums - 1) & 1, LT_TIMEOUT_DRAIN))) break;
         fence_after();
         const uint32_t to = tmem + g % kSums * N, end = min(kRun / kSlab, slabs - run * (kRun / kSlab));
-        for (uint32_t slab = 0; slab < end; ++slab, ++i) {
+        for (uint32_t slab = 0; slab < end; slab += P, ++i) {
           if (!(ok = wait1(&full[i % kDone], i / kDone & 1, LT_TIMEOUT_INPUTS))) break;
           fence_after();
           // A K step of 16 is 32 bytes of each row: 2 in a descriptor's address.
-          const uint64_t xd = xd0 + s * (N * 128 / 16);
-          const uint32_t wa = tmem + kSums * N + 32 * sw;
+          const uint64_t xd = xd0 + s * (P * N * 128 / 16);
+          const uint32_t wa = tmem + kSums * N + 32 * P * sw;
 #pragma unroll
-          for (uint32_t j = 0; j < kSlab / 16; ++j)
-            mma_f16_ts(to, wa + 8 * j, xd + 2 * j, idesc, slab > 0 || j > 0 ? 1u : 0u);
+          for (uint32_t h = 0; h < P; ++h) {
+            if (slab + h >= end) break;
+#pragma unroll
+            for (uint32_t j = 0; j < kSlab / 16; ++j)
+              mma_f16_ts(to, wa + 32 * h + 8 * j, xd + h * (N * 128 / 16) + 2 * j, idesc,
+                         slab > 0 || h > 0 || j > 0 ? 1u : 0u);
+          }
           mma_commit(smem_u32(done_bar(i)));
           s = s + 1 == S ? 0 : s + 1;
           sw = sw + 1 == kWide ? 0 : sw + 1;
