@@ -8,6 +8,8 @@
   (include/furykernel_host.h): programs, plans and launch lists.
 - `furykernel_b200.engine`, `prefill`, `tp`: the decode step, the prompt
   prefill and tensor parallelism on the device.
+- `furykernel_b200.experts`: a routed FFN with MXFP4 experts (grouped route,
+  routed products, gate, combine) for decode rows and prompts.
 """
 
 __version__ = "0.1.0"
