@@ -1,6 +1,6 @@
 """A routed FFN with MXFP4 experts: y = x + sum_j w_j E_ids[j](x).
 
-The router's logits (f32 rows, `gemv`) go through the grouped route, and
+The router's logits (f32, `gemv`, or `gemm_tf32x3w` for many rows) go through the grouped route, and
 each row's experts through the routed MXFP4 products with the GELU gate
 between them; the ranks are combined onto the row. `RoutedExperts` keeps
 the experts' tables at 17 bits to four weights, quantised on the device
@@ -19,6 +19,12 @@ import argparse
 import numpy as np
 
 from furykernel_b200 import _native as N
+
+
+# Rows past which the router is a tensor-core GEMM (the block with 64 experts,
+# 2048 x 1408: 32 rows 190 us by gemv and 198 by GEMM, 64 rows 222 and 206, 511
+# rows 1060 and 335).
+GEMM_ROWS = 48
 
 
 class Mxfp4Table:
@@ -59,6 +65,7 @@ class RoutedExperts:
         self.bias = None if bias is None else ctx.to_device(bias.astype(np.float32))
         self.gate_up = Mxfp4Table(ctx, gate_up, e, 2 * ffn, d)
         self.down = Mxfp4Table(ctx, down, e, d, ffn)
+        self.parts = ctx.empty((2, rows, d)) if rows > GEMM_ROWS else None  # the rows as TF32 parts
         self.logits, self.ids = ctx.zeros((rows, e)), ctx.zeros((rows, top_k), np.uint32)
         self.ws, self.gu = ctx.zeros((rows, top_k)), ctx.zeros((rows, top_k * 2 * ffn))
         self.act, self.out = ctx.zeros((rows, top_k * ffn)), ctx.zeros((rows, top_k * d))
@@ -76,8 +83,12 @@ class RoutedExperts:
         """y [m, d] = x [m, d] + the weighted sum of each row's experts."""
         if not 0 < m <= self.rows:
             raise N.Refused(N.FKC_ERR_ARGUMENT, f"routed experts: {m} rows, outside 1..{self.rows}.")
-        self.ctx.launch("gemv", {"n": self.e, "k": self.d, "m": m, "split": 1, "ldx": self.d, "ldy": self.e},
-                        [self.router, x, self.logits])
+        if m > GEMM_ROWS:
+            self.ctx.launch("gemm_tf32x3w", {"M": m, "N": self.e, "K": self.d, "ldc": self.e},
+                            [x, self.parts, self.parts.at(self.rows * self.d), self.router, self.logits])
+        else:
+            self.ctx.launch("gemv", {"n": self.e, "k": self.d, "m": m, "split": 1, "ldx": self.d, "ldy": self.e},
+                            [self.router, x, self.logits])
         bias = [] if self.bias is None else [self.bias]
         self.ctx.launch("route_grouped_bias" if bias else "route_grouped", {**self.route, "m": m},
                         [self.logits, *bias, self.ids, self.ws])
@@ -87,7 +98,7 @@ class RoutedExperts:
         self.ctx.launch("combine_ranks_add", {"m": m, "k": self.k, "d": self.d}, [x, self.ws, self.out, y])
 
     def free(self) -> None:
-        for b in (self.router, self.bias, self.gate_up, self.down, self.logits, self.ids, self.ws, self.gu, self.act,
+        for b in (self.router, self.bias, self.parts, self.gate_up, self.down, self.logits, self.ids, self.ws, self.gu, self.act,
                   self.out, self.work):
             if b is not None:
                 b.free()
