@@ -40,7 +40,7 @@ constexpr uint32_t kRows = 128;   // weight rows a tile: the MMA's M, TMEM lanes
 constexpr uint32_t kSlab = 64;    // K of a stage: 128 bytes of binary16
 constexpr uint32_t kRun = 512;    // K of a run
 constexpr uint32_t kHalfK = 256;  // K of a stage of codes: 128 bytes, half a run
-constexpr uint32_t kSets = 2;                       // of four widening warps, each a half of every run
+constexpr uint32_t kSets = 2;                       // of four widening warps, each every other run
 constexpr uint32_t kWidenWarps = 4 * kSets;
 constexpr uint32_t kInputWarp = 8 + kWidenWarps, kMmaWarp = kInputWarp + 1, kCodeWarp = kInputWarp + 2;
 constexpr uint32_t kThreads = 32 * (12 + kWidenWarps);
@@ -242,7 +242,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t slabs = (a.kk + kSlab - 1) / kSlab;
-  const uint32_t halves = (a.kk + kHalfK - 1) / kHalfK;
 
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < kDone; ++s) {
@@ -251,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (uint32_t s = 0; s < kCodes; ++s) {
       mbar_init(smem_u32(&rfull[s]), 1);
-      mbar_init(smem_u32(&rempty[s]), kWidenWarps);  // all of them wait for every stage: none may miss its turn
+      mbar_init(smem_u32(&rempty[s]), 4);  // the warps of the set that widens it
     }
     for (uint32_t s = 0; s < 2; ++s) {
       mbar_init(smem_u32(&afull[s]), 1);
@@ -387,107 +386,102 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp < 8 + kWidenWarps) {
     other_registers<TN>();
-    // Widen: a set of four warps takes the first half of every run, the other
-    // the second, a thread a row (its TMEM lane): a slab is 32 bytes of codes
-    // (chunk c of row r's 128 bytes at c ^ (r % 8), the 128-byte swizzle) to
-    // 32 columns of binary16 pairs.
+    // Widen: two sets of four warps, every other run each (a run's scales,
+    // factors and waits take a warp as long as half its slabs: in halves of every
+    // run 33.1 us for 32000 x 4096 by 32 bf16 rows, so 30.6), a thread a
+    // row (its TMEM lane): a slab is 32 bytes of codes (chunk c of row r's 128
+    // bytes at c ^ (r % 8), the 128-byte swizzle) to 32 columns of binary16
+    // pairs.
     const uint32_t id = threadIdx.x - 256, row = id & 127, set = id >> 7, turn = row & 7;
     const uint32_t nb = a.kk / mx::kBlock;
     const uint8_t* from = raw + row * 128;
     const uint32_t to = tmem + ((32 * (warp & 3)) << 16) + kSums * N;
-    uint32_t i0 = 0, q = 0, g = 0;  // steps, stages of codes and runs so far
-    auto scales_of = [&](const Piece& p) {
-      return a.scales + ((size_t)p.e * a.n + min(p.row0 + row, a.n - 1)) * nb;
+    uint32_t i0 = 0, g = 0, run = 0;  // steps and runs so far, run of the piece
+    auto scales = [&]() {
+      return load_scales(a.scales + ((size_t)o.e * a.n + min(o.row0 + row, a.n - 1)) * nb, run * (kRun / mx::kBlock), nb);
     };
     bool ok = true, more = work.next(a, o);
-    const uint8_t* srow = nullptr;
+    auto advance = [&]() {
+      i0 += (min(slabs - run * (kRun / kSlab), kRun / kSlab) + P - 1) / P;
+      ++g;
+      if (++run == o.r1 && (more = work.next(a, o))) run = o.r0;
+    };
+    run = o.r0;
+    if (more && set == 1) advance();
     uint4 next = make_uint4(0, 0, 0, 0);
-    if (more) {
-      srow = scales_of(o);
-      next = load_scales(srow, o.r0 * (kRun / mx::kBlock), nb);
-    }
+    if (more) next = scales();
     while (ok && more) {
-      const Piece p = o;
-      const uint8_t* prow = srow;
-      for (uint32_t run = p.r0; ok && run < p.r1; ++run, ++g) {
-        // A run's scales are loaded one run ahead, the next piece's first too.
-        const uint4 sc = next;
-        if (run + 1 < p.r1) {
-          next = load_scales(prow, (run + 1) * (kRun / mx::kBlock), nb);
-        } else if ((more = work.next(a, o))) {
-          srow = scales_of(o);
-          next = load_scales(srow, o.r0 * (kRun / mx::kBlock), nb);
-        }
-        const int ref = (int)top_scale(sc);
-        if (set == 0) {
-          // The factor back: 2^(ref - 127 - 12).
-          const int p2 = ref - 139;
-          swb[(g % kScaleSlots) * kRows + row] =
-              __uint_as_float(p2 >= -126 ? (uint32_t)(p2 + 127) << 23 : 1u << (p2 + 149));
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&sfull[g % kScaleSlots]));
-        }
-        // This set's eight blocks' scales; and what takes a scale byte to a
-        // binary32 exponent: 2^(byte - ref + 12).
-        const uint32_t mine[2] = {set ? sc.z : sc.x, set ? sc.w : sc.y};
-        const int bias = 139 - ref;
-        const uint32_t left = slabs - run * (kRun / kSlab);  // of the tile
+      // A run's scales are loaded while the set's last one is widened.
+      const uint4 sc = next;
+      const uint32_t at_step = i0, at_run = g, left = slabs - run * (kRun / kSlab);  // slabs of the tile
+      advance();
+      if (more) advance();
+      if (more) next = scales();
+      const int ref = (int)top_scale(sc);
+      // The factor back: 2^(ref - 127 - 12).
+      const int p2 = ref - 139;
+      swb[(at_run % kScaleSlots) * kRows + row] =
+          __uint_as_float(p2 >= -126 ? (uint32_t)(p2 + 127) << 23 : 1u << (p2 + 149));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sfull[at_run % kScaleSlots]));
+      // What takes a scale byte to a binary32 exponent: 2^(byte - ref + 12).
+      const int bias = 139 - ref;
 #pragma unroll 1
-        for (uint32_t half = 0; half < 2 && 4 * half < left; ++half, ++q) {
-          if (!(ok = wait(&rfull[q % kCodes], (q / kCodes) & 1, LT_TIMEOUT_CODES))) break;
-          if (half != set) {
-            if (lane == 0) mbar_arrive(smem_u32(&rempty[q % kCodes]));
-            continue;
-          }
-          const uint8_t* stage = from + (q % kCodes) * kRows * 128;
-          // A step's stores are waited for once a part of the next is widened.
-          auto stored = [&](uint32_t i) {
-            __syncwarp();
-            tmem_wait_st();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&full[i % kDone]));
-          };
-          const uint32_t count = min(left - 4 * half, 4u), first = i0 + 4 / P * half;
-#pragma unroll
-          for (uint32_t h = 0; h < 4; ++h) {
-            if (h >= count) break;
-            const uint32_t i = first + h / P, at = to + 32 * (i % kWide * P + h % P);
-#pragma unroll
-            for (uint32_t c = 0; c < 2; ++c) {
-              const uint4 v = *reinterpret_cast<const uint4*>(stage + (((2 * h + c) ^ turn) << 4));
-              const uint32_t byte = (mine[h / 2] >> (16 * (h % 2) + 8 * c)) & 0xFFu;
-              // Binary16's own range does the rest: subnormal, then 0.
-              const float power = __uint_as_float((uint32_t)max((int)byte + bias, 0) << 23);
-              uint32_t by;
-              asm("cvt.rn.f16x2.f32 %0, %1, %1;" : "=r"(by) : "f"(byte == 255 ? __uint_as_float(0x7FC00000u) : power));
-              const uint32_t words[4] = {v.x, v.y, v.z, v.w};
-              uint32_t wide[16];
-#pragma unroll
-              for (uint32_t u = 0; u < 4; ++u) {
-                uint32_t f[4];
-                mx::widen8_f16(words[u], f);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(wide[4 * u + e]) : "r"(f[e]), "r"(by));
-              }
-              // Half a slab is widened in registers while the last step's
-              // stores are on their way and its columns may be in use.
-              if (c == 0 && h % P == 0) {
-                if (h > 0) stored(i - 1);
-                if (i >= kWide && !(ok = wait(done_bar(i - kWide), (i - kWide) / kDone & 1, LT_TIMEOUT_MMA))) break;
-                fence_after();
-              }
-              __syncwarp();
-              tmem_st16(at + 16 * c, wide);
-            }
-            if (!ok) break;
-          }
-          if (ok) stored(first + (count - 1) / P);
-          if (!ok) break;
+      for (uint32_t half = 0; half < 2; ++half) {
+        const uint32_t q = 2 * at_run + half;
+        if (!(ok = wait(&rfull[q % kCodes], (q / kCodes) & 1, LT_TIMEOUT_CODES))) break;
+        if (4 * half >= left) {  // a stage without codes
           if (lane == 0) mbar_arrive(smem_u32(&rempty[q % kCodes]));
+          break;
         }
-        i0 += (min(left, kRun / kSlab) + P - 1) / P;
+        const uint32_t mine[2] = {half ? sc.z : sc.x, half ? sc.w : sc.y};  // these eight blocks' scales
+        const uint8_t* stage = from + (q % kCodes) * kRows * 128;
+        // A step's stores are waited for once a part of the next is widened.
+        auto stored = [&](uint32_t i) {
+          __syncwarp();
+          tmem_wait_st();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&full[i % kDone]));
+        };
+        const uint32_t count = min(left - 4 * half, 4u), first = at_step + 4 / P * half;
+#pragma unroll
+        for (uint32_t h = 0; h < 4; ++h) {
+          if (h >= count) break;
+          const uint32_t i = first + h / P, at = to + 32 * (i % kWide * P + h % P);
+#pragma unroll
+          for (uint32_t c = 0; c < 2; ++c) {
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + (((2 * h + c) ^ turn) << 4));
+            const uint32_t byte = (mine[h / 2] >> (16 * (h % 2) + 8 * c)) & 0xFFu;
+            // Binary16's own range does the rest: subnormal, then 0.
+            const float power = __uint_as_float((uint32_t)max((int)byte + bias, 0) << 23);
+            uint32_t by;
+            asm("cvt.rn.f16x2.f32 %0, %1, %1;" : "=r"(by) : "f"(byte == 255 ? __uint_as_float(0x7FC00000u) : power));
+            const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+            uint32_t wide[16];
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u) {
+              uint32_t f[4];
+              mx::widen8_f16(words[u], f);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(wide[4 * u + e]) : "r"(f[e]), "r"(by));
+            }
+            // Half a slab is widened in registers while the last step's
+            // stores are on their way and its columns may be in use.
+            if (c == 0 && h % P == 0) {
+              if (h > 0) stored(i - 1);
+              if (i >= kWide && !(ok = wait(done_bar(i - kWide), (i - kWide) / kDone & 1, LT_TIMEOUT_MMA))) break;
+              fence_after();
+            }
+            __syncwarp();
+            tmem_st16(at + 16 * c, wide);
+          }
+          if (!ok) break;
+        }
+        if (ok) stored(first + (count - 1) / P);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive(smem_u32(&rempty[q % kCodes]));
       }
     }
   } else {
@@ -512,16 +506,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     // (or, where a wait ran out, their bytes have come, within limits).
     for (uint32_t j = i > S ? i - S : 0; j < i; ++j) wait1(&full[j % kDone], j / kDone & 1, LT_TIMEOUT_INPUTS);
   } else if (warp == kCodeWarp && elect_one()) {
-    // Codes: half a run a stage.
+    // Codes: half a run a stage, also where a tile's last run has only one.
     uint32_t q = 0;
     bool ok = true;
     while (ok && work.next(a, o))
-      for (uint32_t r = o.r0 * (kRun / kHalfK), end = min(o.r1 * (kRun / kHalfK), halves); r < end; ++r, ++q) {
+      for (uint32_t r = o.r0 * (kRun / kHalfK), end = o.r1 * (kRun / kHalfK); r < end; ++r, ++q) {
         const uint32_t s = q % kCodes;
         if (q >= kCodes && !(ok = wait1(&rempty[s], (q / kCodes - 1) & 1, LT_TIMEOUT_WIDEN))) break;
         const uint32_t bar = smem_u32(&rfull[s]);
-        mbar_expect_tx(bar, kRows * 128);
-        tma_load_3d(smem_u32(raw + s * kRows * 128), &tw, (int)(r * 128), (int)o.row0, (int)o.e, bar);
+        if (r * kHalfK < a.kk) {
+          mbar_expect_tx(bar, kRows * 128);
+          tma_load_3d(smem_u32(raw + s * kRows * 128), &tw, (int)(r * 128), (int)o.row0, (int)o.e, bar);
+        } else {
+          mbar_arrive(bar);
+        }
       }
     for (uint32_t j = q > kCodes ? q - kCodes : 0; j < q; ++j)
       wait1(&rfull[j % kCodes], (j / kCodes) & 1, LT_TIMEOUT_CODES);
