@@ -15,6 +15,13 @@
 // sums. The columns are the inputs: a row as two binary16 parts, x = h1 +
 // h2 relative to the largest of a stage's 256 (within 2^-23 of x or 2^-39
 // of that largest), so 8 columns are 4 rows. Sums of blocks are binary32.
+//
+// Measured (captured launches over weights that are not in L2): 32000 x 4096
+// by one f32 row 20.4 us, 3.4 TB/s of codes and scales, by 4 rows 25.0 us; 64
+// experts of 2816 x 2048, 8 rows' 8 experts each, 41 us, 3.1 TB/s; 1408 x 2048
+// by one row's 4 experts 7.0 us. A launch, the inputs' splitting and the first
+// stages are 5 to 6 us of each; past them 4.4 TB/s, with the SMs issuing in
+// half of their cycles and the warps at each other's sums.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 

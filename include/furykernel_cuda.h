@@ -93,7 +93,9 @@ int fkc_sync(fkc_ctx *ctx);
 /* Synchronizes, then reads and clears the context's device status word:
  * 0, or the code a kernel with bounded waits recorded when one ran out
  * (the tensor-core GEMM: 1 a stage never filled, 2 a stage never freed,
- * 3 the accumulator never completed; the tensor-parallel exchange: 10 + the
+ * 3 the accumulator never completed; the MXFP4 products: 29 a stage of the
+ * few-row kernel's codes never landed, and of the tiled one's 30 inputs, 31
+ * codes, 32 widened weights, 33 products, 34 sums never came; the tensor-parallel exchange: 10 + the
  * exchange buffer whose peers' rows or signal never came). */
 int fkc_status(fkc_ctx *ctx, int *code);
 /* The bound of each wait on another rank (the tensor-parallel exchange's),
