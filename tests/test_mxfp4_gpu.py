@@ -155,6 +155,35 @@ def test_linear(ctx, m, n, k, t):
     assert far <= {"f32": 66 * 2.0 ** -24, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}[t]
 
 
+# Inputs that fill a block's shared memory, and past it; single rows' and short
+# runs of the tiles; two passes over few weights and tiles over many.
+@pytest.mark.parametrize("m,n,k", [(1, 40, 16384), (2, 40, 12288), (3, 48, 5120), (4, 64, 4608), (4, 40, 11008),
+                                   (7, 100, 4352), (8, 33, 1024), (10, 40, 32), (20, 140, 96), (40, 200, 288),
+                                   (70, 260, 800), (150, 129, 1312), (11, 5, 64)])
+@pytest.mark.parametrize("t", TYPES)
+def test_linear_ends(ctx, m, n, k, t):
+    codes, scales = weights(324, n, k)
+    w = X.widen(codes, scales)
+    x = O.normal(325, m * k).reshape(m, k)
+    y = linear(ctx, codes, scales, x, t)
+    xh = held(t, x)
+    assert (np.abs(y - xh @ w.T) <= X.linear_bound(w, xh, t)).all()
+
+
+@pytest.mark.parametrize("m", [6, 8])
+@pytest.mark.parametrize("t", TYPES)
+def test_linear_few_rows_many_weights(ctx, m, t):
+    """Held at some of the columns."""
+    n, k = 16500, 4096
+    codes = O.ints(326, n * k // 2, 256).astype(np.uint8).reshape(n, k // 2)
+    scales = (120 + O.ints(327, n * k // 32, 5)).astype(np.uint8).reshape(n, k // 32)
+    x = O.normal(328, m * k).reshape(m, k)
+    y = linear(ctx, codes, scales, x, t)
+    at = np.unique(np.concatenate([[0, 127, 128, n - 1], O.ints(329, 40, n)]))
+    w, xh = X.widen(codes[at], scales[at]), held(t, x)
+    assert (np.abs(y[:, at] - xh @ w.T) <= X.linear_bound(w, xh, t)).all()
+
+
 @pytest.mark.parametrize("m", [1, 6, 40])
 @pytest.mark.parametrize("t", TYPES)
 def test_linear_strides(ctx, m, t):
