@@ -475,11 +475,11 @@ size_t fk_linear_mxfp4_work(uint64_t entries, uint64_t n, uint64_t kk, uint64_t 
   return 5 * pairs * kk + 16 * (pairs < 512 ? pairs : 512) * n + 16 * pairs + 64 * entries + 65536;
 }
 
-// Weights that are read twice rather than widened by the tile kernel, whose
-// launches and first loads cost more than a second pass over few of them (8
-// rows by 4096 x 4096: 11.1 us in two passes, 20.0 in tiles; 11008 x 4096:
-// 19.3 and 22.5; 32000 x 4096: 42.8 and 32.4).
-constexpr uint64_t kTwice = 64u << 20;
+// Weights read again rather than widened by the tile kernel, whose launches
+// and first loads cost as much as these (8 rows, two passes, by 4096 x 4096:
+// 11.1 us, 20.0 in tiles; by 11008 x 4096 19.3 and 22.5, by 32000 x 4096 42.8
+// and 32.4; 16 rows by 2048 x 2048 8.5 and 12.1, 64 by 1024 x 2048 12.1 and 12.8).
+constexpr uint64_t kAgain = 64u << 20;
 
 cudaError_t fk_launch_linear_mxfp4(const FkLinearMx& a, FkElem e, int sms, int* err, bool pdl, cudaStream_t s) {
   if (a.m == 0 || a.n == 0) return cudaSuccess;
@@ -488,16 +488,21 @@ cudaError_t fk_launch_linear_mxfp4(const FkLinearMx& a, FkElem e, int sms, int* 
     return cudaErrorInvalidValue;
   const uint64_t pairs = (uint64_t)a.m * a.k;
   const uint64_t experts = a.ids && pairs > a.entries ? a.entries : a.ids ? pairs : 1;  // at most
-  // Up to 4 pairs an expert on average, a pass over its weights; up to 8,
-  // two, where the weights are few.
-  if (pairs <= fk::ls::kMaxPairs && a.n >= fk::ls::kTileRows &&
-      (pairs <= 4ull * a.entries || (pairs <= 8ull * a.entries && experts * a.n * a.kk <= kTwice))) {
+  // A pass over an expert's weights for every 4 of its pairs.
+  const uint64_t passes = (pairs + 4 * experts - 1) / (4 * experts);
+  // Routed tiles gain past two (16 experts of 512 x 512, 64 rows' 4 each: 15.5
+  // us in passes, 12.9 in tiles) and over a quarter of the weights (64 experts
+  // of 1024 x 1024, 128 rows' 4 each: 37 us in two, 27.3 in tiles), dense ones
+  // past 16 (500 rows by 1024 x 128: 13.3 us in passes, 8.3 in tiles).
+  if (pairs <= fk::ls::kMaxPairs && a.n >= fk::ls::kTileRows && passes <= (a.ids ? 2 : 16) &&
+      (passes - 1) * experts * a.n * a.kk <= (a.ids ? kAgain / 4 : kAgain)) {
     // Rows a pass: 4, fewer where there are no more or where they do not fit.
     uint32_t R = pairs <= 2 ? (uint32_t)pairs : 4;
     uint32_t share = 0;
     for (; R >= 1; R /= 2) {
-      const uint64_t passes = a.ids ? experts : (pairs + R - 1) / R;
-      share = fk::ls::share_of(passes * ((a.n + fk::ls::kTileRows - 1) / fk::ls::kTileRows), a.kk / 32, R, sms);
+      const uint64_t units = experts * ((pairs + R * experts - 1) / (R * experts)) *
+                             ((a.n + fk::ls::kTileRows - 1) / fk::ls::kTileRows);
+      share = fk::ls::share_of(units, a.kk / 32, R, sms);
       if (share) break;
     }
 #define FK_CALL(E)                                              \

@@ -159,7 +159,8 @@ def test_linear(ctx, m, n, k, t):
 # runs of the tiles; two passes over few weights and tiles over many.
 @pytest.mark.parametrize("m,n,k", [(1, 40, 16384), (2, 40, 12288), (3, 48, 5120), (4, 64, 4608), (4, 40, 11008),
                                    (7, 100, 4352), (8, 33, 1024), (10, 40, 32), (20, 140, 96), (40, 200, 288),
-                                   (70, 260, 800), (150, 129, 1312), (11, 5, 64)])
+                                   (70, 260, 800), (150, 129, 1312), (11, 5, 64),
+                                   (66, 40, 32), (100, 140, 96), (90, 200, 288), (65, 15, 1056)])
 @pytest.mark.parametrize("t", TYPES)
 def test_linear_ends(ctx, m, n, k, t):
     codes, scales = weights(324, n, k)
