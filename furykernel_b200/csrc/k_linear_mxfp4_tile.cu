@@ -45,7 +45,7 @@ namespace lt {
 using namespace tc;
 
 constexpr uint32_t kRows = 128;   // weight rows a tile: the MMA's M, TMEM lanes
-constexpr uint32_t kSlab = 64;    // K of a stage: 128 bytes of binary16
+constexpr uint32_t kSlab = 64;    // K of a slab: 128 bytes of binary16
 constexpr uint32_t kRun = 512;    // K of a run
 constexpr uint32_t kHalfK = 256;  // K of a stage of codes: 128 bytes, half a run
 constexpr uint32_t kSets = 2;                       // of four widening warps, each every other run
@@ -803,14 +803,16 @@ cudaError_t launch_all(const FkLinearMx& a, int sms, int* err, bool pdl, cudaStr
     perm = reinterpret_cast<uint32_t*>(take(4 * pairs));
     slot_of = reinterpret_cast<uint32_t*>(take(4 * pairs));
   }
-  // The token tile that costs least. In units of 2.2 ns: the slabs of an
-  // SM's tiles, whose costs by width are measured (22016 x 4096 by 511 rows:
-  // f32 in tiles of 16, 32, 64 and 128 tokens 531, 281, 184 and 160 us; bf16
-  // of 16, 32, 64 and 160 528, 274, 151 and 100), and the last tiles' sums,
-  // which nothing covers (11008 x 4096 by 128 f32 rows: 64 tokens 31 us, 128
-  // 38; by 64 rows 24 and 45). Routed experts are uneven: half a tile of
-  // each is taken to be empty (64 experts with 32 pairs on average, 2816 x
-  // 2048: 32 tokens 134 us, 64 118, 128 181).
+  // The token tile that costs least: the slabs of an SM's tiles, a slab's
+  // cost by width, and the last tiles' sums, which nothing covers. Measured,
+  // captured: 22016 x 4096 by 511 rows, f32 in tiles of 16, 32, 64 and 128
+  // tokens 412, 233, 166 and 164 us, bf16 of 16, 32, 64 and 160 406, 214, 121
+  // and 103; 11008 x 4096 by 128 f32 rows, 64 tokens 28 us, 128 37, by 64 rows
+  // 22 and 54. The costs count wide tiles for less than those times do, since
+  // call after call runs into the power cap, which narrow tiles, widening more,
+  // meet first. Routed experts are uneven: half a tile of each is taken to be
+  // empty (64 experts with 32 pairs on average, 2816 x 2048: 32 tokens 122 us,
+  // 64 114, 128 186).
   constexpr uint32_t kWidths = 4;
   const uint32_t widths[kWidths] = {16, 32, 64, PARTS == 2 ? 128 : 160};
   const double slab_cost[kWidths] = {100, PARTS == 2 ? 106 : 104, PARTS == 2 ? 139 : 114, PARTS == 2 ? 240 : 151};
