@@ -808,9 +808,9 @@ cudaError_t launch_all(const FkLinearMx& a, int sms, int* err, bool pdl, cudaStr
   // captured: 22016 x 4096 by 511 rows, f32 in tiles of 16, 32, 64 and 128
   // tokens 412, 233, 166 and 164 us, bf16 of 16, 32, 64 and 160 406, 214, 121
   // and 103; 11008 x 4096 by 128 f32 rows, 64 tokens 28 us, 128 37, by 64 rows
-  // 22 and 54. The costs count wide tiles for less than those times do, since
-  // call after call runs into the power cap, which narrow tiles, widening more,
-  // meet first. Routed experts are uneven: half a tile of each is taken to be
+  // 22 and 54. Between widths that are even (the 511 f32 rows, call after
+  // call under the power cap: 64 tokens 179.8 us, 128 178.9) the costs take the
+  // wider one, which widens less. Routed experts are uneven: half a tile of each is taken to be
   // empty (64 experts with 32 pairs on average, 2816 x 2048: 32 tokens 122 us,
   // 64 114, 128 186).
   constexpr uint32_t kWidths = 4;
