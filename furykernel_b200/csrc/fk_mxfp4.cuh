@@ -48,6 +48,23 @@ __device__ __forceinline__ float scale_value(uint32_t s) {
   return __uint_as_float(s == 0 ? 0x00400000u : s == 255 ? 0x7FC00000u : s << 23);
 }
 
+// 2^e, e in -149 .. 127, and the e of such a power.
+__device__ __forceinline__ float power_of_two(int e) {
+  return __uint_as_float(e >= -126 ? (uint32_t)(e + 127) << 23 : 1u << (e + 149));
+}
+__device__ __forceinline__ int exponent_of(float power) {
+  const uint32_t b = __float_as_uint(power);
+  return b >> 23 ? (int)(b >> 23) - 127 : -118 - __clz(b);
+}
+
+// v 2^e + sum, |v| < 2^100, e at most 254, in two steps to the same side: what
+// leaves binary32's range on the way is out of it at the end.
+__device__ __forceinline__ float add_scaled(float v, int e, float sum) {
+  const int at = max(e, -252), half = at >> 1;  // (2^-252 already leaves nothing)
+  return fmaf(__fmul_rn(v, __uint_as_float((uint32_t)(half + 127) << 23)),
+              __uint_as_float((uint32_t)(at - half + 127) << 23), sum);
+}
+
 // Two elements to codes: to nearest, ties to even, past 6 to 6; `lo` in the
 // low half of the byte.
 __device__ __forceinline__ uint32_t narrow2(float lo, float hi) {

@@ -323,33 +323,73 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t p = in_tile >= o.count ? 0 : a.perm ? __ldg(a.perm + slot) : slot;
         place[c] = (uint64_t)(p / a.k) * a.ldy + (uint64_t)(p % a.k) * a.n + o.row0 + 32 * quarter;
       }
+      // The tokens' factors of a run are on their way while the run before it
+      // is added: looked at below, they would hold up the sums by their latency (64
+      // experts of 2816 x 2048 by 2048 x 8 bf16 pairs 298 us so, 266 ahead).
+      constexpr uint32_t kOwn = (kHalf + 31) / 32;
+      float next[kOwn];
+      auto factors = [&](uint32_t run) {
+#pragma unroll
+        for (uint32_t i = 0; i < kOwn; ++i) {
+          const uint32_t c = half * kHalf + lane + 32 * i;
+          next[i] = lane + 32 * i < kHalf && c < o.count ? __ldg(a.sx + (size_t)run * a.slots + o.slot0 + c) : 1.0f;
+        }
+      };
+      factors(o.r0);
       for (uint32_t run = o.r0; run < o.r1; ++run, ++g) {
+        // The weights' factor and the inputs' are powers of two: their product is
+        // exact, or out of binary32's range where a sum times both need not
+        // be (weights of 2^-80 by inputs of 2^-60). `within`: no product is,
+        // as no weights' factor (2^-104 to 2^115) takes one of 2^-45 to 2^12
+        // there. Else the sums take one power after the other, which costs (always:
+        // 22016 x 4096 by 511 f32 rows 253 us, 182 so).
+        bool within = true;
         __syncwarp();
-        for (uint32_t c = lane; c < kHalf; c += 32)
-          mysx[c] = half * kHalf + c < o.count
-                        ? __ldg(a.sx + (size_t)run * a.slots + o.slot0 + half * kHalf + c)
-                        : 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < kOwn; ++i) {
+          if (lane + 32 * i < kHalf) mysx[lane + 32 * i] = next[i];
+          within = within && next[i] >= 0x1p-45f && next[i] <= 0x1p12f;
+        }
+        within = __all_sync(0xffffffffu, within);
         __syncwarp();
+        if (run + 1 < o.r1) factors(run + 1);
         ok = ok && wait(&sfull[g % kScaleSlots], (g / kScaleSlots) & 1, LT_TIMEOUT_WIDEN);
         const float sw = swb[(g % kScaleSlots) * kRows + 32 * quarter + lane];
+        if (!within) {  // large inputs, or a run of tiny ones: by the factors themselves
+          uint32_t low = __float_as_uint(1.0f), high = low;
+          for (uint32_t c = lane; c < kHalf; c += 32)
+            low = min(low, __float_as_uint(mysx[c])), high = max(high, __float_as_uint(mysx[c]));
+          const float least = __uint_as_float(__reduce_min_sync(0xffffffffu, low));
+          const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, high));
+          within = __all_sync(0xffffffffu, __fmul_rn(sw, least) > 0.0f && __fmul_rn(sw, most) < INFINITY);
+        }
         ok = ok && wait(&afull[g % kSums], g / kSums & 1, LT_TIMEOUT_MMA);
         fence_after();
         const uint32_t from = at + g % kSums * N;
         constexpr uint32_t kPiece = kHalf % 16 ? 8 : 16;
+        auto add_run = [&](auto&& add) {
 #pragma unroll
-        for (uint32_t c = 0; c < kHalf; c += kPiece) {
-          uint32_t r0[kPiece], r1[kPiece];
-          if constexpr (PARTS == 2)
-            tmem_ld_pair(from + c, from + TN + c, r0, r1);
-          else
-            tmem_ld_one(from + c, r0);
+          for (uint32_t c = 0; c < kHalf; c += kPiece) {
+            uint32_t r0[kPiece];
+            [[maybe_unused]] uint32_t r1[kPiece];
+            if constexpr (PARTS == 2)
+              tmem_ld_pair(from + c, from + TN + c, r0, r1);
+            else
+              tmem_ld_one(from + c, r0);
 #pragma unroll
-          for (uint32_t j = 0; j < kPiece; ++j) {
-            float v = __uint_as_float(r0[j]);
-            if constexpr (PARTS == 2) v = __fadd_rn(v, __uint_as_float(r1[j]));
-            acc[c + j] = fmaf(v, __fmul_rn(sw, mysx[c + j]), acc[c + j]);
+            for (uint32_t j = 0; j < kPiece; ++j) {
+              float v = __uint_as_float(r0[j]);
+              if constexpr (PARTS == 2) v = __fadd_rn(v, __uint_as_float(r1[j]));
+              acc[c + j] = add(v, mysx[c + j], acc[c + j]);
+            }
           }
-        }
+        };
+        if (within)
+          add_run([&](float v, float sx, float sum) { return fmaf(v, __fmul_rn(sw, sx), sum); });
+        else  // one power after the other
+          add_run([&](float v, float sx, float sum) {
+            return mx::add_scaled(v, mx::exponent_of(sw) + mx::exponent_of(sx), sum);
+          });
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&aempty[g % kSums]));
@@ -425,11 +465,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       advance();
       if (more) advance();
       if (more) next = scales();
-      const int ref = (int)top_scale(sc);
+      // (Relative to 2^(35 - 127) all codes of smaller scales are binary16 still:
+      // rows of zeros, whose scales are 0, have a factor like the others'.)
+      const int ref = max((int)top_scale(sc), 35);
       // The factor back: 2^(ref - 127 - 12).
-      const int p2 = ref - 139;
-      swb[(at_run % kScaleSlots) * kRows + row] =
-          __uint_as_float(p2 >= -126 ? (uint32_t)(p2 + 127) << 23 : 1u << (p2 + 149));
+      swb[(at_run % kScaleSlots) * kRows + row] = mx::power_of_two(ref - 139);
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sfull[at_run % kScaleSlots]));
       // What takes a scale byte to a binary32 exponent: 2^(byte - ref + 12).

@@ -250,6 +250,51 @@ def test_linear_tiny_and_large_inputs(ctx, m):
         assert (np.abs(y - xh @ w.T) <= X.linear_bound(w, xh, "f32")).all()
 
 
+# A scale byte of all weights and the inputs' binade: results at either end of
+# the range, and well inside it where only one of the factors is not.
+RANGE_ENDS = [(0, 30), (2, 0), (20, -10), (60, -60), (116, -113), (10, 100), (140, 80), (236, -3), (247, -60),
+              (254, -100)]
+
+
+@pytest.mark.parametrize("m", [70, 200])
+@pytest.mark.parametrize("byte,binade", RANGE_ENDS)
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_linear_range_ends_in_tiles(ctx, m, byte, binade, t):
+    n, k = 40, 640
+    codes = O.ints(341, n * k // 2, 256).astype(np.uint8).reshape(n, k // 2)
+    scales = np.full((n, k // 32), byte, np.uint8)
+    w = X.widen(codes, scales)
+    x = O.normal(342, m * k).reshape(m, k).astype(np.float64) * 2.0 ** binade
+    xh = held(t, x)
+    y = linear(ctx, codes, scales, x, t)
+    assert (np.abs(y - xh @ w.T) <= X.linear_bound(w, xh, t)).all()
+
+
+def test_linear_zero_codes_of_the_largest_scale_in_tiles(ctx):
+    m, n, k = 70, 20, 128
+    x = O.normal(343, m * k).reshape(m, k).astype(np.float64) * 2.0 ** 120
+    codes, scales = np.zeros((n, k // 2), np.uint8), np.full((n, k // 32), 254, np.uint8)
+    assert (linear(ctx, codes, scales, x, "f32") == 0).all()
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_linear_rows_at_both_ends_in_tiles(ctx, t):
+    """Rows of weights and of inputs over the whole range in one call, held
+    where the sums of magnitudes stay inside it."""
+    m, n, k = 130, 150, 1056
+    codes = O.ints(344, n * k // 2, 256).astype(np.uint8).reshape(n, k // 2)
+    scales = np.repeat(np.linspace(0, 254, n).astype(np.uint8)[:, None], k // 32, 1)
+    x = O.normal(345, m * k).reshape(m, k).astype(np.float64) * np.exp2(np.linspace(-120, 120, m).round())[:, None]
+    w, xh = X.widen(codes, scales), held(t, x)
+    inside = np.abs(xh) @ np.abs(w).T < 2.0 ** 126
+    assert inside.sum() > m * n / 2
+    # bf16's subnormals are 2^-133 apart: half of that for a result below its normal numbers, which
+    # the bound does not have (the exact result, rounded once, is past it at 421 of these places).
+    bound = X.linear_bound(w, xh, t) + {"f32": 0.0, "bf16": 2.0 ** -134}[t]
+    y = linear(ctx, codes, scales, x, t)
+    assert (np.abs(y - xh @ w.T) <= bound)[inside].all()
+
+
 @pytest.mark.parametrize("changed,says", [
     ({"k": 48}, "the dimension k is 48, outside its range 32..65536 multiple of 32"),
     ({"ldx": 63}, "ldx 63 is less than a row's 64 inputs"), ({"ldy": 9}, "ldy 9 is less than a row's 10 outputs"),
