@@ -14,7 +14,9 @@
 // weights, two such products, is one scale, which multiplies the block's
 // sums. The columns are the inputs: a row as two binary16 parts, x = h1 +
 // h2 relative to the largest of a stage's 256 (within 2^-23 of x or 2^-39
-// of that largest), so 8 columns are 4 rows. Sums of blocks are binary32.
+// of that largest), so 8 columns are 4 rows. Sums of blocks are binary32;
+// rows with scales of 2^65 and more, which could take them out of its
+// range before the inputs' power is back, are summed a second time.
 //
 // Measured (captured launches over weights that are not in L2): 32000 x 4096
 // by one f32 row 20.4 us, 3.4 TB/s of codes and scales, by 4 rows 25.0 us; 64
@@ -51,6 +53,9 @@ enum { LS_TIMEOUT = 29 };  // a stage of codes never landed
 // Stages of a warp's own ring.
 constexpr uint32_t kStages = 3;
 
+// What the weights' factors are moved up by, in binades (the smallest scales'
+// products with small inputs keep their bits so); the inputs' take it back.
+constexpr int kMoved = 16;
 // A stage's scale words and their values as factors.
 constexpr uint32_t kScaleBytes = kTileRows * kScaleWords * 4;
 constexpr uint32_t kFactorBytes = kTileRows * kStageBlocks * 4;
@@ -87,6 +92,49 @@ __device__ __forceinline__ void mma0(float (&d)[4], uint32_t a0, uint32_t a1, ui
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// One block of 32: two products of the codes of rows g and g + 8 (four bytes a
+// lane of each) with the inputs' parts, and the rows' sums.
+__device__ __forceinline__ void block_sums(uint32_t codes0, uint32_t codes1, const uint4& x, float& v0, float& v1) {
+  uint32_t p[4], q[4];
+  mx::widen8_f16(codes0, p);
+  mx::widen8_f16(codes1, q);
+  float d[4];
+  mma0(d, p[0], q[0], p[1], q[1], x.x, x.y);
+  mma(d, p[2], q[2], p[3], q[3], x.z, x.w);
+  v0 = __fadd_rn(d[0], d[1]), v1 = __fadd_rn(d[2], d[3]);
+}
+
+// Scale bytes from here on (2^65) may take sums of inputs that were moved up
+// out of binary32's range; 255 is no power.
+constexpr uint32_t kLarge = 192;
+
+// A warp's sums of a unit once more, from global memory, for its rows with
+// large scales: a block's sum takes its own power and the inputs' at once.
+// `codes`, `scales`: row g's, of `blocks` blocks, row g + 8 eight rows on; the
+// warp's blocks are b0 .. b1 - 1, its inputs at xat and sat, its sums at to[0]
+// and to[8] (of lanes that have any).
+__device__ __forceinline__ void sum_large(const uint8_t* codes, const uint8_t* scales, uint32_t blocks, uint32_t b0,
+                                          uint32_t b1, const uint4* xat, const float* sat, uint32_t R, bool any,
+                                          float* to) {
+  float acc[2] = {0.0f, 0.0f};
+  uint32_t top[2] = {0, 0};
+#pragma unroll 1
+  for (uint32_t b = b0; b < b1; ++b, xat += 8 * R) {
+    float v[2];
+    block_sums(__ldg(reinterpret_cast<const uint32_t*>(codes + 16ull * b)),
+               __ldg(reinterpret_cast<const uint32_t*>(codes + 16 * (b + 8ull * blocks))), *xat, v[0], v[1]);
+    const int up = mx::exponent_of(sat[(b - b0) / kStageBlocks * R]) + kMoved - 127;
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+      const uint32_t s = __ldg(scales + b + 8ull * h * blocks);
+      acc[h] = s == 255 ? __uint_as_float(0x7FC00000u) : mx::add_scaled(v[h], (int)s + up, acc[h]);
+      top[h] = max(top[h], s);
+    }
+  }
+  if (any && top[0] >= kLarge) to[0] = acc[0];
+  if (any && top[1] >= kLarge) to[8] = acc[1];
 }
 
 // A pass: up to R pairs of one expert, at `first` of the grouped pairs.
@@ -271,7 +319,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   uint32_t slot = 0, phase = 0, held = 0, shift = 0, tile = u0 % tiles, pass = u0 / tiles;
   bool lost = false;
+  // The lane's blocks of a row's last stage, whose other scales are not the row's.
   const uint32_t ragged = blocks % kStageBlocks;
+  const uint32_t ends = ragged - min(ragged, 4 * (lane & 1)), keep = ends < 4 ? (1u << 8 * ends) - 1 : 0xffffffffu;
+  // Columns without a row take another's (R < 4) or what is there: each
+  // column is its own, and theirs are not stored.
+  const uint4* const x0 = reinterpret_cast<const uint4*>(xs) + (((g >> 1) % R) * 4 + t) * 2 + (g & 1);
+  const float* const sx0 = sxs + t % R;
+  uint32_t large = 0;  // bits 6 and 7 of a scale byte, of the held units' bytes: those of kLarge
   auto group_sync = [&]() {
     if (share > 1)
       asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * share) : "memory");
@@ -306,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint4* to = reinterpret_cast<uint4*>(xs) + ((c * R + r) * 4 + q) * 2;
           to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
           to[1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-          if (lane == 0) sxs[step * R + r] = mx::scale_value((uint32_t)(127 - up));
+          if (lane == 0) sxs[step * R + r] = mx::power_of_two(-up - kMoved);
         }
       }
       __syncwarp();
@@ -314,10 +369,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Where the scale bytes of row lane / 2 lie in their words (a stage moves on by whole words).
     if (tile == 0 || tile + 1 == tiles || u == u0) shift = 8 * ((uint32_t)first_scale(pass, tile, lane >> 1) & 3u);
     float acc0 = 0.0f, acc1 = 0.0f;
-    // Columns without a row take another's (R < 4) or what is there: each
-    // column is its own, and theirs are not stored.
-    const uint4* xat = reinterpret_cast<const uint4*>(xs) + (((g >> 1) % R) * 4 + t) * 2 + (g & 1);
-    const float* sat = sxs + t % R;
+    const uint4* xat = x0;
+    const float* sat = sx0;
     for (uint32_t step = 0; step < steps; ++step) {
       load();
       asm volatile("cp.async.wait_group %0;" ::"n"(stages - 1) : "memory");  // all but the last ones
@@ -327,25 +380,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         record(err, LS_TIMEOUT);
       }
       __syncwarp();
-      // The stage's scales as factors, four blocks of one row a lane: a byte
-      // is its factor's exponent, 0 is 2^-127 and infinity stands for NaN.
+      // The stage's scales as factors, four blocks of one row a lane: 2^(byte -
+      // 127 + kMoved), so that a byte is its factor's exponent. Blocks past
+      // the row's end have zeros for codes and inputs, and any factor.
       {
         const uint32_t* w = reinterpret_cast<const uint32_t*>(mine_smem + slot * kScaleBytes) +
                             (lane >> 1) * kScaleWords + (lane & 1);
-        uint32_t bytes = __funnelshift_r(w[0], w[1], shift);
-        float f[4];
+        uint32_t bytes = __funnelshift_r(w[0], w[1], shift), f[4];
+        if (ragged && s0 + step + 1 == all_steps) bytes &= keep;
+        large |= bytes & (bytes << 1);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float v = fmaxf(__uint_as_float((j < 3 ? bytes << (23 - 8 * j) : bytes >> 1) & 0x7F800000u),
-                                __uint_as_float(0x00400000u));
-          f[j] = fmaf(v, 0.0f, v);
-        }
-        if (ragged && s0 + step + 1 == all_steps) {  // the row ends in this stage: no factor past it
-#pragma unroll
-          for (uint32_t j = 0; j < 4; ++j)
-            if (4 * (lane & 1) + j >= ragged) f[j] = 0.0f;
-        }
-        reinterpret_cast<float4*>(factors)[lane] = make_float4(f[0], f[1], f[2], f[3]);
+        for (int j = 0; j < 4; ++j)
+          f[j] = ((j < 3 ? bytes << (23 - 8 * j) : bytes >> 1) & 0x7F800000u) + ((uint32_t)kMoved << 23);
+        reinterpret_cast<uint4*>(factors)[lane] = make_uint4(f[0], f[1], f[2], f[3]);
       }
       __syncwarp();
       const uint8_t* st = smem + (warp * stages + slot) * kCodeBytes + g * 128 + t * 4;
@@ -357,18 +404,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float s0v[4] = {f0.x, f0.y, f0.z, f0.w}, s1v[4] = {f1.x, f1.y, f1.z, f1.w};
 #pragma unroll
         for (uint32_t bb = 0; bb < 4; ++bb) {
-          // One block of 32: two products, their sums times the block's factors.
           const uint32_t b = b4 + bb;
           const uint8_t* at = st + ((b ^ g) << 4);  // the 128-byte swizzle
-          uint32_t p[4], q[4];
-          mx::widen8_f16(*reinterpret_cast<const uint32_t*>(at), p);
-          mx::widen8_f16(*reinterpret_cast<const uint32_t*>(at + 8 * 128), q);
-          const uint4 x = xat[b * R * 8];
-          float d[4];
-          mma0(d, p[0], q[0], p[1], q[1], x.x, x.y);
-          mma(d, p[2], q[2], p[3], q[3], x.z, x.w);
-          sum0 = fmaf(__fadd_rn(d[0], d[1]), s0v[bb], sum0);
-          sum1 = fmaf(__fadd_rn(d[2], d[3]), s1v[bb], sum1);
+          float v0, v1;  // the block's sums, times its factors
+          block_sums(*reinterpret_cast<const uint32_t*>(at), *reinterpret_cast<const uint32_t*>(at + 8 * 128),
+                     xat[b * R * 8], v0, v1);
+          sum0 = fmaf(v0, s0v[bb], sum0);
+          sum1 = fmaf(v1, s1v[bb], sum1);
         }
       }
       const float sx = *sat;
@@ -378,15 +420,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (++slot == stages) slot = 0, phase ^= 1;
       __syncwarp();  // before the stage is loaded again
     }
-    // The warps' sums of up to `batch` units are added together at once: a
-    // barrier a unit, and the adding behind it, held the warps up for as
-    // long as half a unit's products.
+    // The warps' sums of up to `batch` units of a pass are added together at
+    // once: a barrier a unit, and the adding behind it, held the warps up for
+    // as long as half a unit's products.
     float(*rd)[kTileRows * R] = red[held];
     if (t < (uint32_t)R) {
       rd[warp][t * kTileRows + g] = acc0;
       rd[warp][t * kTileRows + g + 8] = acc1;
     }
-    if (++held < batch && u + 1 < u1) continue;
+    if (++held < batch && u + 1 < u1 && tile + 1 < tiles) continue;
+    // Their rows with large scales are summed again first, while the pass's inputs
+    // are here. (One look for all of them: a vote and a branch a stage cost 3%, one
+    // place of it: a second one, or a call, 2%.)
+    if (__any_sync(0xffffffffu, large & 0x80808080u)) {
+#pragma unroll 1
+      for (uint32_t h = 0; h < held; ++h) {
+        const uint64_t row = (uint64_t)passes[pass].e * a.n + first_row(tile + 1 - held + h) + g;
+        sum_large(a.w + row * (a.kk / 2) + 4 * t, a.scales + row * blocks, blocks, s0 * kStageBlocks,
+                  min((s0 + steps) * kStageBlocks, blocks), x0, sx0, R, t < (uint32_t)R,
+                  &red[h][warp][t * kTileRows + g]);
+      }
+      large = 0;
+    }
     group_sync();
     for (uint32_t o = part * 32 + lane; o < held * (kTileRows * R); o += 32 * share) {
       const uint32_t uo = u + 1 - held + o / (kTileRows * R), i = o % (kTileRows * R);

@@ -270,6 +270,37 @@ def test_linear_range_ends_in_tiles(ctx, m, byte, binade, t):
     assert (np.abs(y - xh @ w.T) <= X.linear_bound(w, xh, t)).all()
 
 
+@pytest.mark.parametrize("m", [1, 2, 4])
+@pytest.mark.parametrize("byte,binade", RANGE_ENDS)
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_linear_range_ends_streamed(ctx, m, byte, binade, t):
+    n, k = 40, 736
+    codes = O.ints(346, n * k // 2, 256).astype(np.uint8).reshape(n, k // 2)
+    scales = np.full((n, k // 32), byte, np.uint8)
+    w = X.widen(codes, scales)
+    x = O.normal(347, m * k).reshape(m, k).astype(np.float64) * 2.0 ** binade
+    xh = held(t, x)
+    y = linear(ctx, codes, scales, x, t)
+    assert (np.abs(y - xh @ w.T) <= X.linear_bound(w, xh, t)).all()
+
+
+def test_linear_large_scales_beside_small_ones_streamed(ctx):
+    """Blocks at both ends of a row and beside other rows, NaN scales among them."""
+    m, n, k = 3, 48, 1120
+    codes = O.ints(348, n * k // 2, 256).astype(np.uint8).reshape(n, k // 2)
+    scales = np.full((n, k // 32), 118, np.uint8)
+    scales[5, 2], scales[5, 9] = 230, 20
+    scales[17, 34], scales[18, 34], scales[40] = 191, 192, 3
+    x = O.normal(349, m * k).reshape(m, k).astype(np.float64) * np.array([1.0, 2.0 ** -60, 2.0 ** -100])[:, None]
+    w, xh = X.widen(codes, scales), held("f32", x)
+    y = linear(ctx, codes, scales, x, "f32")
+    assert (np.abs(y - xh @ w.T) <= X.linear_bound(w, xh, "f32")).all()
+    scales[7, 34] = 255
+    got = linear(ctx, codes, scales, x, "f32")
+    fine = np.arange(n) != 7
+    assert np.isnan(got[:, 7]).all() and np.array_equal(got[:, fine], y[:, fine])
+
+
 def test_linear_zero_codes_of_the_largest_scale_in_tiles(ctx):
     m, n, k = 70, 20, 128
     x = O.normal(343, m * k).reshape(m, k).astype(np.float64) * 2.0 ** 120
