@@ -437,6 +437,37 @@ def test_routed_same_every_time(ctx, m):
         assert np.array_equal(routed(ctx, codes, scales, ids, x, "f32", False), a)
 
 
+@pytest.mark.parametrize("t,entries,n,kk,m,k", [("f32", 8, 256, 2048, 300, 4), ("f32", 3, 520, 2720, 500, 3),
+                                                ("bf16", 8, 700, 2048, 900, 6)])
+def test_routed_same_every_time_over_cut_tiles(ctx, t, entries, n, kk, m, k):
+    """Several token tiles an expert and three and more runs a tile, cut at other
+    runs from tile to tile: where a pair's sums are cut has to be the same."""
+    codes, scales = weights(364, entries, n, kk)
+    ids = O.ints(365, m * k, entries).reshape(m, k)
+    x = O.normal(366, m * kk).reshape(m, kk)
+    a = routed(ctx, codes, scales, ids, x, t, False)
+    for _ in range(8):
+        assert np.array_equal(routed(ctx, codes, scales, ids, x, t, False), a)
+
+
+@pytest.mark.parametrize("entries,m,k", [(1, 700, 1), (31, 513, 2), (1162, 2100, 3), (1163, 2100, 3), (4096, 2111, 8)])
+def test_routed_grouping(ctx, entries, m, k):
+    """Every pair meets its expert, with many experts and few, some of them past the table."""
+    n, kk = 20, 64
+    codes = O.ints(367, entries * n * kk // 2, 256).astype(np.uint8).reshape(entries, n, kk // 2)
+    scales = (120 + O.ints(368, entries * n * kk // 32, 5)).astype(np.uint8).reshape(entries, n, kk // 32)
+    ids = O.ints(369, m * k, entries + entries // 8).reshape(m, k)
+    x = O.normal(370, m * kk).reshape(m, kk)
+    y = routed(ctx, codes, scales, ids, x, "f32", False)
+    w, xh = X.widen(codes, scales), held("f32", x)
+    kept = np.where(ids < entries, ids, 0)
+    want = np.einsum("rjnc,rc->rjn", w[kept], xh) * (ids < entries)[..., None]
+    sums = np.einsum("rjnc,rc->rjn", np.abs(w[kept]), np.abs(xh)) * (ids < entries)[..., None]
+    # One run: at most 4 truncated sums of 2^-23, the inputs' parts 2^-22 (or 2^-38 of the row's largest).
+    top = np.abs(xh).max(-1)[:, None, None] * np.abs(w[kept]).sum(-1)
+    assert (np.abs(y - want) <= sums * 2.0 ** -20 + top * 2.0 ** -38).all()
+
+
 @pytest.mark.parametrize("m", [1, 64])
 def test_routed_past_4_gib(ctx, m):
     """A table whose last expert starts past 2^32 bytes."""
