@@ -84,6 +84,7 @@ def lib() -> ctypes.CDLL:
             "fkc_fnv1a64": (u64, [vp, sz]),
             "fkc_launch": (i32, [vp, i32, vp, sz, vp, i32]),
             "fkc_linear_mxfp4_work": (i32, [u32, u32, u32, u32, u32, ctypes.POINTER(sz)]),
+            "fkc_linear_mxfp4_tokens": (i32, [i32, u32, u32, u32, u32, u32, i32, u32, ctypes.POINTER(u32)]),
             "fkc_capture_begin": (i32, [vp]),
             "fkc_capture_end": (i32, [vp, pvp]),
             "fkc_graph_launch": (i32, [vp, vp]),
@@ -427,6 +428,16 @@ def linear_mxfp4_work(n: int, kk: int, m: int, entries: int = 1, k: int = 1) -> 
     b = ctypes.c_size_t()
     check(lib().fkc_linear_mxfp4_work(entries, n, kk, m, k, ctypes.byref(b)))
     return b.value
+
+
+def linear_mxfp4_tokens(sms: int, n: int, kk: int, m: int, entries: int = 1, k: int = 1, routed: bool = False,
+                        elem_bytes: int = 4) -> int:
+    """The rows of x a tile of the tensor-core kernel that linear_mxfp4 (or
+    `routed`: linear_routed_mxfp4) takes for these sizes, 0: it takes the
+    kernel that streams the weights."""
+    t = ctypes.c_uint32()
+    check(lib().fkc_linear_mxfp4_tokens(sms, entries, n, kk, m, k, int(routed), elem_bytes, ctypes.byref(t)))
+    return t.value
 
 
 def pinned(shape, dtype) -> np.ndarray:

@@ -250,6 +250,10 @@ struct FkLinearMx {
 size_t fk_linear_mxfp4_work(uint64_t entries, uint64_t n, uint64_t kk, uint64_t m, uint64_t k);
 cudaError_t fk_launch_linear_mxfp4(const FkLinearMx& a, FkElem e, int sms, int* err, bool pdl, cudaStream_t s);
 cudaError_t fk_launch_linear_mxfp4_tile(const FkLinearMx& a, FkElem e, int sms, int* err, bool pdl, cudaStream_t s);
+// Which kernel a call takes: the tokens a tile of the tiled one, 0: the streaming
+// one (of its buffers only whether ids is null counts).
+uint32_t fk_linear_mxfp4_tokens(const FkLinearMx& a, FkElem e, int sms);
+uint32_t fk_linear_mxfp4_tile_tokens(const FkLinearMx& a, FkElem e, int sms);
 cudaError_t fk_launch_rope_tables(float* cos_t, float* sin_t, double theta, uint32_t d, uint32_t rotated,
                                   uint32_t positions, cudaStream_t s);
 

@@ -536,11 +536,12 @@ size_t fk_linear_mxfp4_work(uint64_t entries, uint64_t n, uint64_t kk, uint64_t 
 // and 32.4; 16 rows by 2048 x 2048 8.5 and 12.1, 64 by 1024 x 2048 12.1 and 12.8).
 constexpr uint64_t kAgain = 64u << 20;
 
-cudaError_t fk_launch_linear_mxfp4(const FkLinearMx& a, FkElem e, int sms, int* err, bool pdl, cudaStream_t s) {
-  if (a.m == 0 || a.n == 0) return cudaSuccess;
-  if (a.kk == 0 || a.kk % fk::mx::kBlock != 0 || a.k == 0 || a.entries == 0 || a.entries > fk::ls::kMaxEntries ||
-      a.ldx < (uint64_t)a.kk * (a.per_rank ? a.k : 1) || a.ldy < (uint64_t)a.k * a.n)
-    return cudaErrorInvalidValue;
+// The rows a pass of the streaming kernel and the warps a unit for a call; warps
+// 0: the call goes to tiles.
+struct FkStream {
+  uint32_t R, share;
+};
+static FkStream stream_of(const FkLinearMx& a, int sms) {
   const uint64_t pairs = (uint64_t)a.m * a.k;
   const uint64_t experts = a.ids && pairs > a.entries ? a.entries : a.ids ? pairs : 1;  // at most
   // A pass over an expert's weights for every 4 of its pairs.
@@ -549,23 +550,33 @@ cudaError_t fk_launch_linear_mxfp4(const FkLinearMx& a, FkElem e, int sms, int* 
   // us in passes, 12.9 in tiles) and over a quarter of the weights (64 experts
   // of 1024 x 1024, 128 rows' 4 each: 37 us in two, 27.3 in tiles), dense ones
   // past 16 (500 rows by 1024 x 128: 13.3 us in passes, 8.3 in tiles).
-  if (pairs <= fk::ls::kMaxPairs && a.n >= fk::ls::kTileRows && passes <= (a.ids ? 2 : 16) &&
-      (passes - 1) * experts * a.n * a.kk <= (a.ids ? kAgain / 4 : kAgain)) {
-    // Rows a pass: 4, fewer where there are no more or where they do not fit.
-    uint32_t R = pairs <= 2 ? (uint32_t)pairs : 4;
-    uint32_t share = 0;
-    for (; R >= 1; R /= 2) {
-      const uint64_t units = experts * ((pairs + R * experts - 1) / (R * experts)) *
-                             ((a.n + fk::ls::kTileRows - 1) / fk::ls::kTileRows);
-      share = fk::ls::share_of(units, a.kk / 32, R, sms);
-      if (share) break;
-    }
-#define FK_CALL(E)                                              \
-  (R == 1   ? fk::ls::launch<E, 1>(a, share, sms, err, pdl, s)   \
-   : R == 2 ? fk::ls::launch<E, 2>(a, share, sms, err, pdl, s)   \
-            : fk::ls::launch<E, 4>(a, share, sms, err, pdl, s))
-    if (share) return FK_BY_ELEM(e, FK_CALL);
-#undef FK_CALL
+  if (pairs > fk::ls::kMaxPairs || a.n < fk::ls::kTileRows || passes > (a.ids ? 2 : 16) ||
+      (passes - 1) * experts * a.n * a.kk > (a.ids ? kAgain / 4 : kAgain))
+    return {0, 0};
+  // Rows a pass: 4, fewer where there are no more or where they do not fit.
+  for (uint32_t R = pairs <= 2 ? (uint32_t)pairs : 4; R >= 1; R /= 2) {
+    const uint64_t units = experts * ((pairs + R * experts - 1) / (R * experts)) *
+                           ((a.n + fk::ls::kTileRows - 1) / fk::ls::kTileRows);
+    if (const uint32_t share = fk::ls::share_of(units, a.kk / 32, R, sms)) return {R, share};
   }
-  return fk_launch_linear_mxfp4_tile(a, e, sms, err, pdl, s);
+  return {0, 0};
+}
+
+uint32_t fk_linear_mxfp4_tokens(const FkLinearMx& a, FkElem e, int sms) {
+  return stream_of(a, sms).share ? 0 : fk_linear_mxfp4_tile_tokens(a, e, sms);
+}
+
+cudaError_t fk_launch_linear_mxfp4(const FkLinearMx& a, FkElem e, int sms, int* err, bool pdl, cudaStream_t s) {
+  if (a.m == 0 || a.n == 0) return cudaSuccess;
+  if (a.kk == 0 || a.kk % fk::mx::kBlock != 0 || a.k == 0 || a.entries == 0 || a.entries > fk::ls::kMaxEntries ||
+      a.ldx < (uint64_t)a.kk * (a.per_rank ? a.k : 1) || a.ldy < (uint64_t)a.k * a.n)
+    return cudaErrorInvalidValue;
+  const FkStream v = stream_of(a, sms);
+  if (!v.share) return fk_launch_linear_mxfp4_tile(a, e, sms, err, pdl, s);
+#define FK_CALL(E)                                                  \
+  (v.R == 1   ? fk::ls::launch<E, 1>(a, v.share, sms, err, pdl, s)   \
+   : v.R == 2 ? fk::ls::launch<E, 2>(a, v.share, sms, err, pdl, s)   \
+              : fk::ls::launch<E, 4>(a, v.share, sms, err, pdl, s))
+  return FK_BY_ELEM(e, FK_CALL);
+#undef FK_CALL
 }

@@ -850,6 +850,35 @@ cudaError_t launch_tile(const FkLinearMx& a, const fk::lt::Args& g, const uint16
                       smem < 120 * 1024 ? (size_t)120 * 1024 : smem, s, pdl, tx, tw, g, (long long)4000000000LL, err);
 }
 
+// A call's tokens a tile, inputs in so many parts.
+uint32_t token_tile(const FkLinearMx& a, int parts, int sms) {
+  // The token tile that costs least: the slabs of an SM's tiles, a slab's
+  // cost by width, and the last tiles' sums, which nothing covers. Measured,
+  // captured: 22016 x 4096 by 511 rows, f32 in tiles of 16, 32, 64 and 128
+  // tokens 412, 233, 166 and 164 us, bf16 of 16, 32, 64 and 160 406, 214, 121
+  // and 103; 11008 x 4096 by 128 f32 rows, 64 tokens 28 us, 128 37, by 64 rows
+  // 22 and 54. Between widths that are even (the 511 f32 rows, call after
+  // call under the power cap: 64 tokens 179.8 us, 128 178.9) the costs take the
+  // wider one, which widens less. Routed experts are uneven: half a tile of each is taken to be
+  // empty (64 experts with 32 pairs on average, 2816 x 2048: 32 tokens 122 us,
+  // 64 114, 128 186).
+  const uint64_t pairs = (uint64_t)a.m * a.k, wtiles = (a.n + fk::lt::kRows - 1) / fk::lt::kRows;
+  constexpr uint32_t kWidths = 4;
+  const uint32_t widths[kWidths] = {16, 32, 64, parts == 2 ? 128u : 160u};
+  const double slab_cost[kWidths] = {100, parts == 2 ? 106. : 104., parts == 2 ? 139. : 114., parts == 2 ? 240. : 151.};
+  const double used = pairs < a.entries ? (double)pairs : (double)a.entries;
+  const double slabs = used * wtiles * ((a.kk + fk::lt::kSlab - 1) / fk::lt::kSlab) / sms;
+  uint32_t tn = 16;
+  double least = 0;
+  for (uint32_t i = 0; i < kWidths; ++i) {
+    const double share = (double)pairs / used / widths[i];
+    const double tiles = !a.ids ? (double)((pairs + widths[i] - 1) / widths[i]) : share > 0.5 ? share + 0.5 : 1.0;
+    const double cost = tiles * slabs * slab_cost[i] + 70.0 * widths[i];
+    if (i == 0 || cost < least) least = cost, tn = widths[i];
+  }
+  return tn;
+}
+
 template <class E, int PARTS>
 cudaError_t launch_all(const FkLinearMx& a, int sms, int* err, bool pdl, cudaStream_t s) {
   using namespace fk::lt;
@@ -874,30 +903,7 @@ cudaError_t launch_all(const FkLinearMx& a, int sms, int* err, bool pdl, cudaStr
     perm = reinterpret_cast<uint32_t*>(take(4 * pairs));
     slot_of = reinterpret_cast<uint32_t*>(take(4 * pairs));
   }
-  // The token tile that costs least: the slabs of an SM's tiles, a slab's
-  // cost by width, and the last tiles' sums, which nothing covers. Measured,
-  // captured: 22016 x 4096 by 511 rows, f32 in tiles of 16, 32, 64 and 128
-  // tokens 412, 233, 166 and 164 us, bf16 of 16, 32, 64 and 160 406, 214, 121
-  // and 103; 11008 x 4096 by 128 f32 rows, 64 tokens 28 us, 128 37, by 64 rows
-  // 22 and 54. Between widths that are even (the 511 f32 rows, call after
-  // call under the power cap: 64 tokens 179.8 us, 128 178.9) the costs take the
-  // wider one, which widens less. Routed experts are uneven: half a tile of each is taken to be
-  // empty (64 experts with 32 pairs on average, 2816 x 2048: 32 tokens 122 us,
-  // 64 114, 128 186).
-  constexpr uint32_t kWidths = 4;
-  const uint32_t widths[kWidths] = {16, 32, 64, PARTS == 2 ? 128 : 160};
-  const double slab_cost[kWidths] = {100, PARTS == 2 ? 106 : 104, PARTS == 2 ? 139 : 114, PARTS == 2 ? 240 : 151};
-  const uint32_t wtiles = (a.n + kRows - 1) / kRows;
-  const double used = pairs < a.entries ? (double)pairs : (double)a.entries;
-  const double slabs = used * wtiles * ((a.kk + kSlab - 1) / kSlab) / sms;
-  uint32_t tn = 16;
-  double least = 0;
-  for (uint32_t i = 0; i < kWidths; ++i) {
-    const double share = (double)pairs / used / widths[i];
-    const double tiles = !a.ids ? (double)((pairs + widths[i] - 1) / widths[i]) : share > 0.5 ? share + 0.5 : 1.0;
-    const double cost = tiles * slabs * slab_cost[i] + 70.0 * widths[i];
-    if (i == 0 || cost < least) least = cost, tn = widths[i];
-  }
+  const uint32_t tn = token_tile(a, PARTS, sms), wtiles = (a.n + kRows - 1) / kRows;
   if (a.ids) {
     const uint32_t chunk = (uint32_t)((pairs + 32 * sms - 1) / (32 * sms)) * 32;
     cudaError_t e = fk_launch_ex(group_kernel, dim3((uint32_t)((pairs + chunk - 1) / chunk)), dim3(1024), 0, s, pdl,
@@ -936,6 +942,10 @@ cudaError_t launch_all(const FkLinearMx& a, int sms, int* err, bool pdl, cudaStr
 }
 
 }  // namespace
+
+uint32_t fk_linear_mxfp4_tile_tokens(const FkLinearMx& a, FkElem e, int sms) {
+  return token_tile(a, e == FK_F32 ? 2 : 1, sms);
+}
 
 cudaError_t fk_launch_linear_mxfp4_tile(const FkLinearMx& a, FkElem e, int sms, int* err, bool pdl, cudaStream_t s) {
   if (a.entries > fk::lt::kMaxEntries) return cudaErrorInvalidValue;

@@ -1719,6 +1719,18 @@ extern "C" int fkc_linear_mxfp4_work(uint32_t entries, uint32_t n, uint32_t kk, 
   return FKC_OK;
 }
 
+extern "C" int fkc_linear_mxfp4_tokens(int sms, uint32_t entries, uint32_t n, uint32_t kk, uint32_t m, uint32_t k,
+                                       int routed, uint32_t elem_bytes, uint32_t* tokens) {
+  if (!tokens || sms < 1 || !entries || !n || !kk || !m || !k || kk % 32 != 0 || (elem_bytes != 2 && elem_bytes != 4))
+    return fail(FKC_ERR_ARGUMENT, "fkc_linear_mxfp4_tokens: bad argument.");
+  static const uint32_t any = 0;
+  FkLinearMx a = {};
+  a.ids = routed ? &any : nullptr;
+  a.entries = entries, a.n = n, a.kk = kk, a.m = m, a.k = k;
+  *tokens = fk_linear_mxfp4_tokens(a, elem_bytes == 4 ? FK_F32 : FK_BF16, sms);
+  return FKC_OK;
+}
+
 // ---------------------------------------------------------------------------
 // Graphs
 

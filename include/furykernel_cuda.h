@@ -180,6 +180,12 @@ int fkc_launch(fkc_ctx *ctx, int kernel, const void *params, size_t params_len, 
  * 5 m k kk + 16 min(m k, 512) n + 16 m k + 64 entries + 65536. The launch
  * writes it before it reads it; what it holds between launches is nobody's. */
 int fkc_linear_mxfp4_work(uint32_t entries, uint32_t n, uint32_t kk, uint32_t m, uint32_t k, size_t *bytes);
+/* Which of their two kernels these products take on a GPU of `sms` SMs, x and y
+ * of elem_bytes (4 f32, 2 bf16 or f16): *tokens is the rows of x a tile of
+ * the tensor-core kernel, or 0 for the kernel that streams the weights. For
+ * tests and tuning: the results' accuracy is the same. */
+int fkc_linear_mxfp4_tokens(int sms, uint32_t entries, uint32_t n, uint32_t kk, uint32_t m, uint32_t k, int routed,
+                            uint32_t elem_bytes, uint32_t *tokens);
 
 /* ---- the tree reduction without allocation --------------------------------- */
 /* No counterpart in the reference. The sum of n f32 values at x into *y, with

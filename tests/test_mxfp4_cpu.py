@@ -70,3 +70,15 @@ def test_packing_words_a_wrong_name():
         e.pack({"n": 1, "k": 32, "m": 1, "ldx": 32})
     assert e.pack({"ldy": 5, "ldx": 4, "m": 3, "k": 32, "n": 1}) == b"".join(
         v.to_bytes(4, "little") for v in (1, 32, 3, 4, 5))
+
+
+def test_which_kernel():
+    """One row streams, a prompt goes to the widest tiles; the tests of each kernel state their own sizes."""
+    import pytest
+
+    assert N.linear_mxfp4_tokens(148, 11008, 4096, 1) == 0
+    assert [N.linear_mxfp4_tokens(148, 22016, 4096, 511, elem_bytes=b) for b in (4, 2)] == [128, 160]
+    assert N.linear_mxfp4_tokens(148, 1408, 2048, 1, 64, 4, True) == 0
+    for bad in ((0, 64, 64, 1), (148, 64, 48, 1), (148, 64, 64, 0), (148, 64, 64, 1, 1, 1, False, 1)):
+        with pytest.raises(N.Refused, match="fkc_linear_mxfp4_tokens: bad argument"):
+            N.linear_mxfp4_tokens(*bad)

@@ -261,6 +261,7 @@ RANGE_ENDS = [(0, 30), (2, 0), (20, -10), (60, -60), (116, -113), (10, 100), (14
 @pytest.mark.parametrize("t", ["f32", "bf16"])
 def test_linear_range_ends_in_tiles(ctx, m, byte, binade, t):
     n, k = 40, 640
+    assert tokens(ctx, n, k, m, t) > 0
     codes = O.ints(341, n * k // 2, 256).astype(np.uint8).reshape(n, k // 2)
     scales = np.full((n, k // 32), byte, np.uint8)
     w = X.widen(codes, scales)
@@ -275,6 +276,7 @@ def test_linear_range_ends_in_tiles(ctx, m, byte, binade, t):
 @pytest.mark.parametrize("t", ["f32", "bf16"])
 def test_linear_range_ends_streamed(ctx, m, byte, binade, t):
     n, k = 40, 736
+    assert tokens(ctx, n, k, m, t) == 0
     codes = O.ints(346, n * k // 2, 256).astype(np.uint8).reshape(n, k // 2)
     scales = np.full((n, k // 32), byte, np.uint8)
     w = X.widen(codes, scales)
@@ -287,6 +289,7 @@ def test_linear_range_ends_streamed(ctx, m, byte, binade, t):
 def test_linear_large_scales_beside_small_ones_streamed(ctx):
     """Blocks at both ends of a row and beside other rows, NaN scales among them."""
     m, n, k = 3, 48, 1120
+    assert tokens(ctx, n, k, m, "f32") == 0
     codes = O.ints(348, n * k // 2, 256).astype(np.uint8).reshape(n, k // 2)
     scales = np.full((n, k // 32), 118, np.uint8)
     scales[5, 2], scales[5, 9] = 230, 20
@@ -303,6 +306,7 @@ def test_linear_large_scales_beside_small_ones_streamed(ctx):
 
 def test_linear_zero_codes_of_the_largest_scale_in_tiles(ctx):
     m, n, k = 70, 20, 128
+    assert tokens(ctx, n, k, m, "f32") > 0
     x = O.normal(343, m * k).reshape(m, k).astype(np.float64) * 2.0 ** 120
     codes, scales = np.zeros((n, k // 2), np.uint8), np.full((n, k // 32), 254, np.uint8)
     assert (linear(ctx, codes, scales, x, "f32") == 0).all()
@@ -313,6 +317,7 @@ def test_linear_rows_at_both_ends_in_tiles(ctx, t):
     """Rows of weights and of inputs over the whole range in one call, held
     where the sums of magnitudes stay inside it."""
     m, n, k = 130, 150, 1056
+    assert tokens(ctx, n, k, m, t) > 0
     codes = O.ints(344, n * k // 2, 256).astype(np.uint8).reshape(n, k // 2)
     scales = np.repeat(np.linspace(0, 254, n).astype(np.uint8)[:, None], k // 32, 1)
     x = O.normal(345, m * k).reshape(m, k).astype(np.float64) * np.exp2(np.linspace(-120, 120, m).round())[:, None]
@@ -442,6 +447,7 @@ def test_routed_same_every_time(ctx, m):
 def test_routed_same_every_time_over_cut_tiles(ctx, t, entries, n, kk, m, k):
     """Several token tiles an expert and three and more runs a tile, cut at other
     runs from tile to tile: where a pair's sums are cut has to be the same."""
+    assert tokens(ctx, n, kk, m, t, entries, k, True) * entries < m * k
     codes, scales = weights(364, entries, n, kk)
     ids = O.ints(365, m * k, entries).reshape(m, k)
     x = O.normal(366, m * kk).reshape(m, kk)
@@ -498,6 +504,111 @@ def test_routed_past_4_gib(ctx, m):
     assert (y[:, n:] == 0).all()
     for b in (wd, sd, idd, xd, yd, work):
         b.free()
+
+
+# --------------------------------------------------------------------------
+# Each kernel by name: the sizes state which one they reach, and a change of the
+# rule that sends them elsewhere fails here.
+
+
+def tokens(ctx, n, k, m, t, entries=1, ranks=1, routed=False):
+    from furykernel_b200 import _native as N
+
+    return N.linear_mxfp4_tokens(ctx.sms, n, k, m, entries, ranks, routed, 4 if t == "f32" else 2)
+
+
+def any_weights(seed, *shape):
+    """Codes of every kind, scales over 5 binades."""
+    size = int(np.prod(shape))
+    codes = O.ints(seed, size // 2, 256).astype(np.uint8).reshape(shape[:-1] + (-1,))
+    return codes, (116 + O.ints(seed + 1, size // 32, 5)).astype(np.uint8).reshape(shape[:-1] + (-1,))
+
+
+def some_columns(seed, n):
+    return np.unique(np.concatenate([[0, min(127, n - 1), min(128, n - 1), n - 1], O.ints(seed, 40, n)]))
+
+
+# By norm, as test_linear: 66 steps of 2^-24, 16-bit outputs their own rounding.
+NORM = {"f32": 66 * 2.0 ** -24, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}
+# (rows, n, k, tokens a tile: f32, 16-bit)
+DENSE_TILES = [(70, 300, 1120, 16, 16), (65, 2100, 4128, 32, 32), (128, 4500, 4128, 64, 64), (500, 8900, 4128, 128, 160)]
+
+
+@pytest.mark.parametrize("m,n,k,wide,narrow", DENSE_TILES)
+@pytest.mark.parametrize("t", TYPES)
+def test_linear_tiles(ctx, m, n, k, wide, narrow, t):
+    """Every width of tile, tiles cut over the blocks, rows and columns off the
+    tiles' ends, rows off 16 bytes."""
+    assert tokens(ctx, n, k, m, t) == (wide if t == "f32" else narrow)
+    codes, scales = any_weights(401, n, k)
+    x = O.normal(403, m * k).reshape(m, k) * np.exp(O.normal(404, k))[None]
+    y = linear(ctx, codes, scales, x, t)
+    assert np.array_equal(linear(ctx, codes, scales, x, t, k + 1, n + 3), y)
+    at = some_columns(405, n)
+    w, xh = X.widen(codes[at], scales[at]), held(t, x)
+    want = xh @ w.T
+    assert (np.abs(y[:, at] - want) <= X.linear_bound(w, xh, t)).all()
+    assert np.linalg.norm(y[:, at] - want) / np.linalg.norm(want) <= NORM[t]
+
+
+@pytest.mark.parametrize("m,n,k,wide,narrow", DENSE_TILES)
+@pytest.mark.parametrize("t", TYPES)
+def test_linear_tiles_tiny_and_large_inputs(ctx, m, n, k, wide, narrow, t):
+    """Rows of inputs over the type's range, zeros, an infinity and a NaN among them."""
+    assert tokens(ctx, n, k, m, t) == (wide if t == "f32" else narrow)
+    codes, scales = any_weights(406, n, k)
+    ends = 8 if t == "f16" else 100
+    x = O.normal(408, m * k).reshape(m, k) * np.exp2(np.linspace(-ends, ends, m).round())[:, None]
+    x[7] = 0
+    x[20, 600], x[m - 1, 0] = np.inf, np.nan
+    y = linear(ctx, codes, scales, x, t)
+    at = some_columns(409, n)
+    w, xh = X.widen(codes[at], scales[at]), held(t, x)
+    fine = np.isfinite(xh).all(-1)
+    assert fine.sum() == m - 2
+    assert (np.abs(y[fine][:, at] - xh[fine] @ w.T) <= X.linear_bound(w, xh[fine], t)).all()
+    assert (y[7] == 0).all() and np.isnan(y[m - 1]).all()
+    with np.errstate(invalid="ignore"):
+        assert np.array_equal(y[20, at], np.inf * w[:, 600], equal_nan=True)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 300, 1120), (2, 2100, 608), (3, 130, 4128), (40, 48, 640), (40, 77, 352)])
+@pytest.mark.parametrize("t", TYPES)
+def test_linear_streamed(ctx, m, n, k, t):
+    assert tokens(ctx, n, k, m, t) == 0
+    codes, scales = any_weights(411, n, k)
+    x = O.normal(413, m * k).reshape(m, k) * np.exp(O.normal(414, k))[None]
+    y = linear(ctx, codes, scales, x, t)
+    assert np.array_equal(linear(ctx, codes, scales, x, t, k + 1, n + 3), y)
+    w, xh = X.widen(codes, scales), held(t, x)
+    want = xh @ w.T
+    assert (np.abs(y - want) <= X.linear_bound(w, xh, t)).all()
+    assert np.linalg.norm(y - want) / np.linalg.norm(want) <= NORM[t]
+
+
+@pytest.mark.parametrize("entries,n,kk,m,k,wide,narrow", [
+    (8, 300, 1120, 2, 3, 0, 0), (4, 260, 544, 300, 3, 16, 16), (8, 900, 2080, 200, 4, 32, 32),
+    (8, 900, 2080, 300, 8, 64, 64), (2, 7000, 4128, 900, 2, 128, 160)])
+@pytest.mark.parametrize("per_rank", [False, True])
+@pytest.mark.parametrize("t", TYPES)
+def test_routed_kernels(ctx, entries, n, kk, m, k, wide, narrow, per_rank, t):
+    """As test_linear_tiles, with some ids past the table; held at some of the columns."""
+    assert tokens(ctx, n, kk, m, t, entries, k, True) == (wide if t == "f32" else narrow)
+    codes, scales = any_weights(421, entries, n, kk)
+    ids = O.ints(423, m * k, entries).reshape(m, k)
+    ids[m - 1, 0] = entries
+    width = kk * (k if per_rank else 1)
+    x = O.normal(424, m * width).reshape(m, width)
+    y = routed(ctx, codes, scales, ids, x, t, per_rank, width + 1, k * n + 3)
+    at = some_columns(425, n)
+    held_to_experts(y[:, :, at], codes[:, at], scales[:, at], ids, x, t, per_rank)
+    w, xh = X.widen(codes[:, at], scales[:, at]), held(t, x).reshape(m, -1, kk)
+    off = total = 0.0
+    for r, j in np.argwhere(ids < entries):
+        want = w[ids[r, j]] @ xh[r, j if per_rank else 0]
+        off += ((y[r, j, at] - want) ** 2).sum()
+        total += (want ** 2).sum()
+    assert np.sqrt(off / total) <= NORM[t]
 
 
 def test_routed_refusals(ctx):
