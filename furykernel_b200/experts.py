@@ -58,6 +58,8 @@ class RoutedExperts:
                  groups: int = 1, top_groups: int = 1, group_by: int = 1, sigmoid: bool = False,
                  renorm: bool = True, factor: float = 1.0, bias: np.ndarray = None):
         e, d = router.shape
+        if bias is not None and bias.size != e:
+            raise N.Refused(N.FKC_ERR_ARGUMENT, f"routed experts: the bias has {bias.size} values, not {e}.")
         self.ctx, self.e, self.d, self.ffn, self.k, self.rows = ctx, e, d, ffn, top_k, rows
         self.route = {"n": e, "k": top_k, "groups": groups, "top_groups": top_groups, "group_by": group_by,
                       "sigmoid": int(sigmoid), "renorm": int(renorm), "ldx": e, "factor": factor}
@@ -83,6 +85,9 @@ class RoutedExperts:
         """y [m, d] = x [m, d] + the weighted sum of each row's experts."""
         if not 0 < m <= self.rows:
             raise N.Refused(N.FKC_ERR_ARGUMENT, f"routed experts: {m} rows, outside 1..{self.rows}.")
+        for name, b in (("x", x), ("y", y)):
+            if isinstance(b, N.DeviceBuffer) and b.nbytes < 4 * m * self.d:
+                raise N.Refused(N.FKC_ERR_ARGUMENT, f"routed experts: {name} holds fewer than {m} rows of {self.d}.")
         if m > GEMM_ROWS:
             self.ctx.launch("gemm_tf32x3w", {"M": m, "N": self.e, "K": self.d, "ldc": self.e},
                             [x, self.parts, self.parts.at(self.rows * self.d), self.router, self.logits])

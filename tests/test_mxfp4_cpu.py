@@ -60,6 +60,26 @@ def test_forms_retype_the_activations():
                 assert b.type == (t if a.name in typed else a.type)
 
 
+def test_routed_experts_refuse_buffers_that_are_too_short():
+    """Before anything is allocated or launched: what is read past its end would be another's memory."""
+    import pytest
+
+    from furykernel_b200.experts import RoutedExperts
+
+    e, d, ffn = 8, 64, 32
+    arrays = np.zeros((e, d)), np.zeros((e, 2 * ffn, d)), np.zeros((e, d, ffn))
+    for short in (e - 1, e + 1, 1):
+        with pytest.raises(N.Refused, match=f"routed experts: the bias has {short} values, not 8"):
+            RoutedExperts(None, *arrays, ffn, 2, 4, bias=np.zeros(short))
+    block = object.__new__(RoutedExperts)
+    block.rows, block.d = 4, d
+    rows = [N.DeviceBuffer(None, 256, 4 * n * d) for n in (2, 3)]
+    with pytest.raises(N.Refused, match="routed experts: x holds fewer than 3 rows of 64"):
+        block.launch(rows[0], rows[1], 3)
+    with pytest.raises(N.Refused, match="routed experts: y holds fewer than 3 rows of 64"):
+        block.launch(rows[1], rows[0], 3)
+
+
 def test_packing_words_a_wrong_name():
     import pytest
 
