@@ -83,6 +83,38 @@ def test_experts_block(ctx, m, bias):
     yd.free()
 
 
+@pytest.mark.parametrize("m", [5, 70])
+def test_experts_block_captured(ctx, m):
+    """A graph of the block computes all of it from the rows that it finds: every buffer
+    between the rows and the result is marked before each replay, and the rows change."""
+    b = block(ctx, 300, True)[0]
+    xd, yd = ctx.zeros((m, D)), ctx.zeros((m, D))
+    rows = [O.normal(506 + i, m * D).reshape(m, D).astype(np.float32) for i in range(3)]
+    xd.upload(rows[0])
+    ctx.capture_begin()
+    b.launch(xd, yd, m)
+    g = ctx.capture_end()
+    eager = []
+    for x in rows:
+        xd.upload(x)
+        b.launch(xd, yd, m)
+        eager.append((yd.download(), b.ids.download()[:m]))
+    assert not np.array_equal(eager[0][1], eager[1][1])
+    for x, (y, ids) in zip(rows, eager):
+        xd.upload(x)
+        for between in (b.logits, b.ids, b.ws, b.gu, b.act, b.out, b.work, b.parts, yd):
+            between.upload(np.full(between.shape, 0x7F, between.dtype))
+        g.launch()
+        ctx.sync()
+        assert np.array_equal(yd.download(), y)
+        assert np.array_equal(b.ids.download()[:m], ids)
+    assert ctx.status() == 0
+    g.destroy()
+    b.free()
+    xd.free()
+    yd.free()
+
+
 def test_refusals(ctx):
     from furykernel_b200 import _native as N
     from furykernel_b200.experts import Mxfp4Table
