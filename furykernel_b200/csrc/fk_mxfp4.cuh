@@ -32,17 +32,6 @@ __device__ __forceinline__ void widen8_f16(uint32_t w, uint32_t (&d)[4]) {
       : "r"(w));
 }
 
-__device__ __forceinline__ void widen8(uint32_t w, float (&v)[8]) {
-  uint32_t h[4];
-  widen8_f16(w, h);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = F16::widen2(h[i]);
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
-}
-
 // A scale byte's value: 2^(s - 127), subnormal at s = 0, NaN at s = 255.
 __device__ __forceinline__ float scale_value(uint32_t s) {
   return __uint_as_float(s == 0 ? 0x00400000u : s == 255 ? 0x7FC00000u : s << 23);

@@ -317,7 +317,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (uint32_t c = 0; c < kHalf; ++c) acc[c] = 0.0f;
       __syncwarp();
-      __syncwarp();
       for (uint32_t c = lane; c < kHalf; c += 32) {
         const uint32_t in_tile = half * kHalf + c, slot = o.slot0 + in_tile;
         const uint32_t p = in_tile >= o.count ? 0 : a.perm ? __ldg(a.perm + slot) : slot;
