@@ -19,8 +19,8 @@
 // range before the inputs' power is back, are summed a second time.
 //
 // Measured (captured launches over weights that are not in L2): 32000 x 4096
-// by one f32 row 20.4 us, 3.4 TB/s of codes and scales, by 4 rows 25.0 us; 64
-// experts of 2816 x 2048, 8 rows' 8 experts each, 41 us, 3.1 TB/s; 1408 x 2048
+// by one f32 row 20.6 us, 3.4 TB/s of codes and scales, by 4 rows 25.2 us; 64
+// experts of 2816 x 2048, 8 rows' 8 experts each, 37 us, 3.4 TB/s; 1408 x 2048
 // by one row's 4 experts 7.0 us. A launch, the inputs' splitting and the first
 // stages are 5 to 6 us of each; past them 4.4 TB/s, with the SMs issuing in
 // half of their cycles and the warps at each other's sums.
@@ -470,7 +470,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 // How many warps share a unit: the fewest rounds of units, each its blocks
 // a warp and about 8 blocks' worth of fixed cost, and the inputs' splitting
 // before them, whose inputs fit (4096 x 11008 by one row: 16 warps 11.4 us, 8
-// 12.9). 0: none.
+// 12.9). Each group of warps has its own copy of the inputs, so at 4 rows a pass
+// it is often shared memory that decides: K = 1408 leaves 8 warps a unit, where
+// the costs alone would take 2. 0: none.
 inline uint32_t share_of(uint64_t units, uint32_t blocks, uint32_t R, int sms) {
   uint32_t best = 0;
   uint64_t least = ~0ull;
@@ -532,8 +534,8 @@ size_t fk_linear_mxfp4_work(uint64_t entries, uint64_t n, uint64_t kk, uint64_t 
 
 // Weights read again rather than widened by the tile kernel, whose launches
 // and first loads cost as much as these (8 rows, two passes, by 4096 x 4096:
-// 11.1 us, 20.0 in tiles; by 11008 x 4096 19.3 and 22.5, by 32000 x 4096 42.8
-// and 32.4; 16 rows by 2048 x 2048 8.5 and 12.1, 64 by 1024 x 2048 12.1 and 12.8).
+// 11.4 us, 19.2 in tiles; by 11008 x 4096 19.5 and 21.1, by 32000 x 4096 44.1
+// and 30.0; 16 rows by 2048 x 2048 8.3 and 12.7, 64 by 1024 x 2048 12.3 and 13.0).
 constexpr uint64_t kAgain = 64u << 20;
 
 // The rows a pass of the streaming kernel and the warps a unit for a call; warps
@@ -546,10 +548,10 @@ static FkStream stream_of(const FkLinearMx& a, int sms) {
   const uint64_t experts = a.ids && pairs > a.entries ? a.entries : a.ids ? pairs : 1;  // at most
   // A pass over an expert's weights for every 4 of its pairs.
   const uint64_t passes = (pairs + 4 * experts - 1) / (4 * experts);
-  // Routed tiles gain past two (16 experts of 512 x 512, 64 rows' 4 each: 15.5
-  // us in passes, 12.9 in tiles) and over a quarter of the weights (64 experts
-  // of 1024 x 1024, 128 rows' 4 each: 37 us in two, 27.3 in tiles), dense ones
-  // past 16 (500 rows by 1024 x 128: 13.3 us in passes, 8.3 in tiles).
+  // Routed tiles gain past two (16 experts of 512 x 512, 64 rows' 4 each: 15.3
+  // us in passes, 13.4 in tiles) and over a quarter of the weights (64 experts
+  // of 1024 x 1024, 128 rows' 4 each: 38 us in two, 31 in tiles), dense ones
+  // past 16 (500 rows by 1024 x 128: 13.3 us in passes, 8.5 in tiles).
   if (pairs > fk::ls::kMaxPairs || a.n < fk::ls::kTileRows || passes > (a.ids ? 2 : 16) ||
       (passes - 1) * experts * a.n * a.kk > (a.ids ? kAgain / 4 : kAgain))
     return {0, 0};

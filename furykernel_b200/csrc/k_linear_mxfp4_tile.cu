@@ -6,16 +6,17 @@
 // of two moves a binary16 within its 40 binades without rounding, so the
 // products run as kind::f16 with binary32 accumulators: K moves in runs of
 // 512, in each run a weight row's scales are taken relative to the row's
-// largest there (2^12 of it; a scale more than 2^36 below loses bits of
-// values under 2^-36 of the largest), and a row's inputs relative to their
-// largest in the run (2^14 of it). f32 inputs go as two binary16 parts, x =
-// h1 + h2 within 2^-23 of x or 2^-39 of the run's largest, side by side as
-// N columns of one instruction; bf16 and f16 inputs are one part, exact but
-// for bf16 values 2^-38 below the run's largest. Both factors return when a
-// run's sums leave the tensor memory for f32 registers. Runs are short for
-// one more reason: the tensor cores cut each accumulation off instead of
-// rounding it, which over all of K = 4096 cost 3xTF32 products 1.4e-5 of
-// the result, always toward zero; over the 32 steps of a run it is 5e-7.
+// largest there (2^12 of it; codes of scales 2^36 and more below it lose bits),
+// and a row's inputs relative to their largest in the run (2^14 of it). f32
+// inputs go as two binary16 parts, x = h1 + h2 within 2^-23 of x or 2^-39 of
+// the run's largest, side by side as N columns of one instruction; f16 inputs
+// are one part, as they are, and bf16 inputs one, whole down to 2^-31 of the
+// run's largest and within 2^-39 of it below. Both factors return when a run's
+// sums leave the tensor memory for f32 registers. Runs are short for one more
+// reason: the tensor cores cut each accumulation off instead of rounding it. Sums
+// of 4096 positive products come out 6.7e-6 of the result too small from the TF32
+// GEMM, which adds all of K in place, and 2.3e-7 from the 32 steps of a run here, at
+// K = 512 and at 4096.
 //
 // Three launches:
 //   group   the pairs of each expert in order, their slots in expert order, the
@@ -24,13 +25,13 @@
 //           slot order, and their factors; pairs without an expert get zeros;
 //   tile    persistent CTAs over (expert, token tile, 128 weight rows).
 //
-// Measured (captured launches): 22016 x 4096 by 511 f32 rows 160 us, 576
-// TFLOP/s (two products each), the tensor pipe 61 to 65% busy at
-// the 1.6 to 1.8 GHz that the power cap leaves; by 511 bf16 rows 99 us; 32000 x
-// 4096 by 32 bf16 rows 30.6 us; 64 experts of 2816 x 2048, 2048 bf16 rows' 8
-// each, 290 us, 650 TFLOP/s. Tiles of 64 and fewer tokens are bound by the
-// widening warps (about 2800 cycles a run of 512 x 128 weights), wider ones
-// by the MMAs.
+// Measured (captured calls): 22016 x 4096 by 511 f32 rows 152 us, 606 TFLOP/s
+// (two products each), and 171 us where calls follow one another under the
+// power cap, the tensor pipe 61 to 66% busy; by 511 bf16 rows 100 and 111 us; 32000 x 4096
+// by 32 bf16 rows 31.8 us; 64 experts of 2816 x 2048, 2048 bf16 rows' 8 each, 266
+// and 296 us, of which group 6 and split 15, the tensor pipe 50 to 55% busy. Tiles
+// of 64 and fewer tokens are bound by the widening warps (about 2800 cycles a run
+// of 512 x 128 weights).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -853,14 +854,13 @@ cudaError_t launch_tile(const FkLinearMx& a, const fk::lt::Args& g, const uint16
 uint32_t token_tile(const FkLinearMx& a, int parts, int sms) {
   // The token tile that costs least: the slabs of an SM's tiles, a slab's
   // cost by width, and the last tiles' sums, which nothing covers. Measured,
-  // captured: 22016 x 4096 by 511 rows, f32 in tiles of 16, 32, 64 and 128
-  // tokens 412, 233, 166 and 164 us, bf16 of 16, 32, 64 and 160 406, 214, 121
-  // and 103; 11008 x 4096 by 128 f32 rows, 64 tokens 28 us, 128 37, by 64 rows
-  // 22 and 54. Between widths that are even (the 511 f32 rows, call after
-  // call under the power cap: 64 tokens 179.8 us, 128 178.9) the costs take the
-  // wider one, which widens less. Routed experts are uneven: half a tile of each is taken to be
-  // empty (64 experts with 32 pairs on average, 2816 x 2048: 32 tokens 122 us,
-  // 64 114, 128 186).
+  // captured, call after call: 22016 x 4096 by 511 rows, f32 in tiles of 16,
+  // 32, 64 and 128 tokens 412, 247, 176 and 172 us, bf16 of 16, 32, 64 and 160
+  // 404, 216, 133 and 111; 11008 x 4096 by 128 f32 rows, 64 tokens 30 us, 128
+  // 35, by 65 rows 30 and 39 (32 tokens 32). Between widths that are even the
+  // costs take the wider one, which widens less. Routed experts are uneven:
+  // half a tile of each is taken to be empty (64 experts with 32 pairs on
+  // average, 2816 x 2048: 32 tokens 123 us, 64 118, 128 185).
   const uint64_t pairs = (uint64_t)a.m * a.k, wtiles = (a.n + fk::lt::kRows - 1) / fk::lt::kRows;
   constexpr uint32_t kWidths = 4;
   const uint32_t widths[kWidths] = {16, 32, 64, parts == 2 ? 128u : 160u};

@@ -23,7 +23,7 @@ from furykernel_b200 import _native as N
 
 # Rows past which the router is a tensor-core GEMM (the block with 64 experts,
 # 2048 x 1408: 32 rows 188 us by gemv and 199 by GEMM, 64 rows 200 and 186, 511
-# rows 1032 and 319).
+# rows 1032 and 318).
 GEMM_ROWS = 48
 
 
